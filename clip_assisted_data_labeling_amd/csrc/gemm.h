@@ -58,6 +58,13 @@ struct GemmParams {
 #endif
 };
 
+#ifdef __HIPCC__
+// the next number of a launch's tile counter, for one lane; agent scope: the workgroups of all XCDs count on the same word
+__device__ __forceinline__ unsigned take_ticket(unsigned* counter) {
+  return __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+#endif
+
 hipError_t ce_gemm_nt(const GemmParams& p, int dtype, int epi, hipStream_t stream);
 hipError_t ce_gemm_fp8(const GemmParams& p, int epi, hipStream_t stream);           // fp8 e4m3 operands; EPI_STORE_BF16 / EPI_RESID / EPI_STORE_FP8 / EPI_RESID_Q
 hipError_t ce_gemm_nt_persist(const GemmParams& p, int epi, hipStream_t stream);   // bf16; EPI_STORE_BF16 / LNFOLD / RESID

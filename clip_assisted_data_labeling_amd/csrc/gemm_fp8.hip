@@ -160,7 +160,7 @@ __global__ __launch_bounds__(512, 2) void gemm_fp8_kernel(const GemmParams p) {
 #define DECODE_TILE(i_) (EPI == 4 ? tri_tile(p.tile_list, (i_)) : decode_tile((i_), tiles_m, tiles_n))
   const int G = gridDim.x;
   // Dynamic tail (p.ticket; gemm_persist.hip has the argument and the measurements): the tiles from S on -- the launch's last
-  // one-to-two rounds -- are taken from a global ticket counter (a scalar atomic: lgkmcnt, not the DMA pipeline's vmcnt) in the
+  // one-to-two rounds -- are taken from a global ticket counter (a vector atomic by one lane) in the
   // order the workgroups get there.  The ticket waits in word 512 of wave 4's image: [2048, 2560) of an image is written by no
   // DMA piece of any instantiation, and the epilogue, which owns the whole image, starts after the ticket has been read.
 #ifndef F8_DYN_ROUNDS
@@ -380,21 +380,19 @@ __global__ __launch_bounds__(512, 2) void gemm_fp8_kernel(const GemmParams p) {
 #endif
     if (wr == 1) {
       if (EPI != 4 && w == 4 && idx + G >= S) {             // the tile after this one comes from the ticket counter
-        int cand = -1;
-        if (by_xcd) {
-          for (int j = 0; j < 8 && cand < 0; ++j) {
-            const int x = (blockIdx.x + j) & 7;
-            unsigned tk = 1;
-            asm volatile("s_atomic_add %0, %1, 0x0 glc\n\ts_waitcnt lgkmcnt(0)" : "+s"(tk) : "s"(p.ticket + x) : "memory");
-            const int id = S + (int)tk * 8 + x;
-            if ((unsigned)id < (unsigned)nwg) cand = id;
+        if (lane == 0) {
+          int cand = -1;
+          if (by_xcd) {
+            for (int j = 0; j < 8 && cand < 0; ++j) {
+              const int x = (blockIdx.x + j) & 7;
+              const int id = S + (int)take_ticket(p.ticket + x) * 8 + x;
+              if ((unsigned)id < (unsigned)nwg) cand = id;
+            }
+          } else {
+            cand = S + (int)take_ticket(p.ticket);
           }
-        } else {
-          unsigned tk = 1;
-          asm volatile("s_atomic_add %0, %1, 0x0 glc\n\ts_waitcnt lgkmcnt(0)" : "+s"(tk) : "s"(p.ticket) : "memory");
-          cand = S + (int)tk;
+          *(volatile __attribute__((address_space(3))) int*)LDS_PTR(TICKET_SLOT) = cand;
         }
-        if (lane == 0) *(volatile __attribute__((address_space(3))) int*)LDS_PTR(TICKET_SLOT) = cand;
       }
       BARRIER();                             // second wave row runs half a phase behind
     }

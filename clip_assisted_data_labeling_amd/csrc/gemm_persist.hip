@@ -142,9 +142,10 @@ __global__ __launch_bounds__(512, 2) void gemm_persist_kernel(const GemmParams p
   // S on -- between one and two rounds -- are taken from a global ticket counter in the order the workgroups arrive.  The
   // workgroups of a launch drift apart (tools/gemm_stamps.py: finish times spread over more than a tile time; mean idle at the end
   // of a launch 2-3.4 %, of which the static partial round is 0.4-2.7 %), and with tickets the ones that run ahead take the extra
-  // tiles.  The ticket is a SCALAR atomic (s_atomic_add, counted in lgkmcnt): a vector atomic would join the in-order vmcnt
-  // queue that the DMA pipeline's hand-counted waits are written against.  One wave takes it at the top of a tile, a tile
-  // before it is needed, and parks it in a free word of its epilogue image; which workgroup runs a tile changes no result bit.
+  // tiles.  The ticket is a vector atomic by one lane: it joins the in-order vmcnt queue behind the DMA pipeline's loads, and the
+  // wait for its answer drains them too, so that the pipeline's hand-counted waits, which count what is issued later, only find
+  // less outstanding than they allow for.  One wave takes it at the top of a tile, a tile before it is needed, and parks it in a
+  // free word of its epilogue image; which workgroup runs a tile changes no result bit.
   // Two forms (measured, tools/experiments/README.md): outputs of 4 tiles along N (out-proj, FC2) -- ONE counter, one full round
   // by ticket; wider outputs (QKV, FC1: 12 / 16 tiles along N, whose XCD-aware order is worth 0.5 % on two ticketed rounds) -- one
   // counter PER XCD (p.ticket[0..7]), two full rounds: the workgroups of XCD x take the positions of ITS strided sequence (tile
@@ -379,21 +380,19 @@ __global__ __launch_bounds__(512, 2) void gemm_persist_kernel(const GemmParams p
       }
       if (EPI != EPI_THRESH && w == 4 && idx + G >= S) {
         // the tile after this one comes from the ticket counters: take the ticket now (~1 us; this wave row waits here anyway)
-        int cand = -1;
-        if (by_xcd) {
-          for (int j = 0; j < 8 && cand < 0; ++j) {
-            const int x = (blockIdx.x + j) & 7;
-            unsigned tk = 1;
-            asm volatile("s_atomic_add %0, %1, 0x0 glc\n\ts_waitcnt lgkmcnt(0)" : "+s"(tk) : "s"(p.ticket + x) : "memory");
-            const int id = S + (int)tk * 8 + x;
-            if ((unsigned)id < (unsigned)nwg) cand = id;
+        if (lane == 0) {
+          int cand = -1;
+          if (by_xcd) {
+            for (int j = 0; j < 8 && cand < 0; ++j) {
+              const int x = (blockIdx.x + j) & 7;
+              const int id = S + (int)take_ticket(p.ticket + x) * 8 + x;
+              if ((unsigned)id < (unsigned)nwg) cand = id;
+            }
+          } else {
+            cand = S + (int)take_ticket(p.ticket);
           }
-        } else {
-          unsigned tk = 1;
-          asm volatile("s_atomic_add %0, %1, 0x0 glc\n\ts_waitcnt lgkmcnt(0)" : "+s"(tk) : "s"(p.ticket) : "memory");
-          cand = S + (int)tk;
+          *(volatile int*)(smem + TICKET_SLOT) = cand;
         }
-        if (lane == 0) *(volatile int*)(smem + TICKET_SLOT) = cand;
       }
       BARRIER();                             // second wave row runs half a phase behind
     }
