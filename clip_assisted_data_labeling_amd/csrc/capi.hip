@@ -282,7 +282,7 @@ int run_tower(clipenc_s* e, const void* crops, int c, int in_dtype, int n_layers
   };
   // ticket counters of this pass's persistent GEMM launches (at most 6 per block + the patch GEMM): zeroed by one fill
   int tk = 0;
-  if (e->dynamic_tail) HIP_TRY(hipMemsetAsync(e->tickets, 0, CE_TICKET_WORDS * sizeof(unsigned), st));
+  if (e->dynamic_tail) HIP_TRY(ce_clear_words(e->tickets, CE_TICKET_WORDS, st));
   auto ticket = [&]() -> unsigned* { return (e->dynamic_tail && (tk + 1) * 8 <= CE_TICKET_WORDS) ? e->tickets + 8 * tk++ : nullptr; };
   // The LAST block's attention for the class-token query without K and V (cls_attention.hip): r_h = (Q_cls masked to head h) . W'_k
   // and o_h = z_h . W'_v^T as two small launches of the persistent GEMM (16 x redundant -- every head's row against every column --
@@ -1156,7 +1156,7 @@ int dedup_find_pairs(const void* emb_f16_dev, int n, int d, float threshold, int
   if (n < 0 || d < 1) return fail("dedup_find_pairs: bad shape n=%d d=%d", n, d);
   if (!count_dev) return fail("dedup_find_pairs: count_dev is NULL");
   hipStream_t st = (hipStream_t)stream;
-  HIP_TRY(hipMemsetAsync(count_dev, 0, sizeof(unsigned long long), st));
+  HIP_TRY(ce_clear_words(count_dev, 2, st));
   if (n < 2) return 0;
   if (!emb_f16_dev || !ehat_ws_dev || (capacity && (!pairs_dev || !vals_dev))) return fail("dedup_find_pairs: NULL device pointer");
   const int ld = (d + 127) / 128 * 128;
@@ -1192,7 +1192,7 @@ int dedup_find_pairs_screened(const void* emb_f16_dev, int n, int d, float thres
   if (n < 0 || d < 1) return fail("dedup_find_pairs_screened: bad shape n=%d d=%d", n, d);
   if (!count_dev) return fail("dedup_find_pairs_screened: count_dev is NULL");
   hipStream_t st = (hipStream_t)stream;
-  HIP_TRY(hipMemsetAsync(count_dev, 0, sizeof(unsigned long long), st));
+  HIP_TRY(ce_clear_words(count_dev, 2, st));
   if (n < 2) return 0;
   if (!emb_f16_dev || !ehat_ws_dev || !screen_ws_dev || (capacity && (!pairs_dev || !vals_dev))) return fail("dedup_find_pairs_screened: NULL device pointer");
   if (candidate_capacity < 1) return fail("dedup_find_pairs_screened: candidate_capacity must be at least 1");

@@ -229,7 +229,7 @@ hipError_t ce_dedup_normalize_f16(const void* emb_f16, void* out_f16, int n, int
 hipError_t ce_dedup_normalize_quant(const void* emb_f16, void* out_f16, int n, int d, int ld, void* q8_ws, int ld8, float* margin_ws,
                                     unsigned long long* cand_count, unsigned long long cand_cap, hipStream_t stream) {
   const int n_pad = (n + 255) / 256 * 256;
-  if (hipError_t e = hipMemsetAsync(cand_count, 0, sizeof(unsigned long long), stream); e != hipSuccess) return e;
+  if (hipError_t e = ce_clear_words(cand_count, 2, stream); e != hipSuccess) return e;
   if (d % 8 == 0 && ld % 8 == 0 && ld8 % 8 == 0 && !(((uintptr_t)emb_f16 | (uintptr_t)out_f16 | (uintptr_t)q8_ws) & 15)) {
     hipLaunchKernelGGL(dedup_normalize_quant_kernel, dim3((n_pad + 3) / 4), dim3(256), 0, stream, (const _Float16*)emb_f16, (_Float16*)out_f16, n, d,
                        n_pad, ld, (unsigned char*)q8_ws, ld8, margin_ws, cand_count, cand_cap + 1);

@@ -493,3 +493,16 @@ hipError_t ce_gather_row_stats(const float* in, int in_ld, float* out, int out_l
                      out_ld, n, row_stride);
   return hipGetLastError();
 }
+
+// Counters are cleared by a kernel and not by hipMemsetAsync: the calls that clear them may be captured into a graph, and memset
+// nodes have been seen to give wrong results on replays after the first.
+__global__ void clear_words_kernel(unsigned* __restrict__ p, int n) {
+  const int i = blockIdx.x * blockDim.x + threadIdx.x;
+  if (i < n) p[i] = 0u;
+}
+
+hipError_t ce_clear_words(void* p, int n_words, hipStream_t stream) {
+  if (n_words < 1) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(clear_words_kernel, dim3((n_words + 255) / 256), dim3(256), 0, stream, (unsigned*)p, n_words);
+  return hipGetLastError();
+}

@@ -573,8 +573,7 @@ __global__ __launch_bounds__(512, 2) void gemm_persist_kernel(const GemmParams p
         const float mean = t.x, rstd = t.y;
 #pragma unroll
         for (int nt = 0; nt < 4; ++nt) {
-          // whole-vector arithmetic so that hipcc emits v_pk_fma / v_pk_mul / v_pk_add (two elements per instruction);
-          // only exp2 and rcp stay per element
+          // whole-vector arithmetic, so that the exp2 and the rcp of the four elements stand apart from their consumers
           f32x4_t v = rstd * (acc[mt][nt] - mean * cs[nt]) + bs[nt];
           if constexpr (ACT == CE_ACT_QUICK_GELU) {
             f32x4_t t = v * -2.4554669595930156f;
