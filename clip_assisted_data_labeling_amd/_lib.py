@@ -99,6 +99,15 @@ SIGNATURES = {
                                         c_void_p, c_int, c_void_p, c_void_p, c_void_p]),
     "clipenc_op_gemm_fp8_resid_q": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                             c_void_p, c_int, c_void_p]),
+    "clipenc_op_quant_mx": (c_int, [c_void_p, c_int, c_long, c_int, c_long, c_int, c_void_p, c_void_p, c_void_p]),
+    "clipenc_op_dequant_mx": (c_int, [c_void_p, c_void_p, c_int, c_long, c_int, c_void_p, c_int, c_void_p]),
+    "clipenc_op_norm_quant_mx": (c_int, [c_void_p, c_int, c_long, c_int, c_long, c_void_p, c_long, c_int, c_void_p, c_void_p, c_float, c_int,
+                                         c_void_p, c_void_p, c_void_p, c_void_p]),
+    "clipenc_op_gemm_mx": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p,
+                                   c_int, c_void_p]),
+    "clipenc_op_linear_mx_ws_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "clipenc_op_linear_mx": (c_int, [c_void_p, c_int, c_long, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_void_p,
+                                     c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
     "clipenc_forward_tokens": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p]),
     "jpegdec_create": (c_int, [c_int, c_void_p]),
     "jpegdec_destroy": (c_int, [c_void_p]),

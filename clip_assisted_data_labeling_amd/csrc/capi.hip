@@ -19,6 +19,7 @@
 #include "gemm.h"
 #include "jpeg_host.h"
 #include "kernels.h"
+#include "mx.h"
 
 namespace {
 
@@ -1357,6 +1358,125 @@ int clipenc_op_gemm_fp8_q(const void* a8_dev, const void* w8_dev, int m, int n, 
   hipError_t err = ce_gemm_fp8(p, EPI_STORE_FP8, (hipStream_t)stream);
   if (err != hipSuccess) return fail("gemm_fp8_q(%d,%d,%d) failed: %s", m, n, k, hipGetErrorString(err));
   return 0;
+}
+
+// ---- microscaled rows (mx.h) ----
+namespace {
+bool aligned_to(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+size_t dt_size(int dtype) { return dtype == CLIPENC_DT_F32 ? 4 : 2; }
+bool dt_known(int dtype) { return dtype == CLIPENC_DT_BF16 || dtype == CLIPENC_DT_F16 || dtype == CLIPENC_DT_F32; }
+constexpr int MX_MAX_K = 1 << 20;
+
+int mx_check_rows(const char* what, const void* in, int dtype, long n_rows, int k, long ld) {
+  if (n_rows < 0 || k < 1 || k > MX_MAX_K) return fail("%s: %ld rows of %d columns (k = 1 .. %d)", what, n_rows, k, MX_MAX_K);
+  if (!dt_known(dtype)) return fail("%s: in_dtype = %d (CLIPENC_DT_*)", what, dtype);
+  if (ld < k) return fail("%s: rows of %d columns lie %ld elements apart", what, k, ld);
+  if (n_rows && !in) return fail("%s: NULL device pointer", what);
+  if (!aligned_to(in, dt_size(dtype))) return fail("%s: rows not aligned to their type", what);
+  return 0;
+}
+int mx_check_q(const char* what, const void* q, const void* scale) {
+  if (!q || !scale) return fail("%s: NULL device pointer", what);
+  if (!aligned_to(q, 16) || !aligned_to(scale, 4)) return fail("%s: elements are 16-byte aligned, scales 4-byte", what);
+  return 0;
+}
+int mx_check_product(const char* what, const void* w, const void* w_scale, int m, int n, int k, const float* bias, int act, const void* resid,
+                     const void* out, int out_dtype) {
+  if (m < 0 || n < 0 || k < 1 || k > MX_MAX_K) return fail("%s: bad shape m=%d n=%d k=%d (k = 1 .. %d)", what, m, n, k, MX_MAX_K);
+  if (!dt_known(out_dtype)) return fail("%s: out_dtype = %d (CLIPENC_DT_*)", what, out_dtype);
+  if (act != -1 && act != CLIPENC_ACT_QUICK_GELU && act != CLIPENC_ACT_GELU_ERF) return fail("%s: act = %d", what, act);
+  if (resid && act != -1) return fail("%s: activation and residual are exclusive", what);
+  if (m == 0 || n == 0) return 0;
+  if (int rc = mx_check_q(what, w, w_scale)) return rc;
+  if (!out) return fail("%s: NULL device pointer", what);
+  if (!aligned_to(bias, 4) || !aligned_to(out, dt_size(out_dtype)) || !aligned_to(resid, dt_size(out_dtype))) return fail("%s: a pointer is not aligned to its type", what);
+  return 0;
+}
+size_t mx_row_bytes(int k, int fmt) { return fmt == CLIPENC_MX_E2M1 ? (size_t)mx_kp(k) / 2 : (size_t)mx_kp(k); }
+}  // namespace
+
+int clipenc_op_quant_mx(const void* in_dev, int in_dtype, long n_rows, int k, long ld_in, int fmt, void* out_dev, void* scale_dev,
+                        void* stream) {
+  if (int rc = mx_check_rows("quant_mx", in_dev, in_dtype, n_rows, k, ld_in)) return rc;
+  if (fmt != CLIPENC_MX_E2M1 && fmt != CLIPENC_MX_E4M3) return fail("quant_mx: fmt = %d (CLIPENC_MX_E2M1 or CLIPENC_MX_E4M3)", fmt);
+  if (n_rows == 0) return 0;
+  if (int rc = mx_check_q("quant_mx", out_dev, scale_dev)) return rc;
+  hipError_t err = ce_mx_quant(in_dev, in_dtype, n_rows, k, ld_in, fmt, (uint8_t*)out_dev, (uint8_t*)scale_dev, (hipStream_t)stream);
+  if (err != hipSuccess) return fail("quant_mx(%ld,%d) failed: %s", n_rows, k, hipGetErrorString(err));
+  return 0;
+}
+
+int clipenc_op_dequant_mx(const void* q_dev, const void* scale_dev, int fmt, long n_rows, int k, void* out_dev, int out_dtype,
+                          void* stream) {
+  if (n_rows < 0 || k < 1 || k > MX_MAX_K) return fail("dequant_mx: %ld rows of %d columns (k = 1 .. %d)", n_rows, k, MX_MAX_K);
+  if (fmt < CLIPENC_MX_E2M1 || fmt > CLIPENC_ROW_E4M3) return fail("dequant_mx: fmt = %d", fmt);
+  if (!dt_known(out_dtype)) return fail("dequant_mx: out_dtype = %d (CLIPENC_DT_*)", out_dtype);
+  if (n_rows == 0) return 0;
+  if (int rc = mx_check_q("dequant_mx", q_dev, scale_dev)) return rc;
+  if (!out_dev || !aligned_to(out_dev, dt_size(out_dtype))) return fail("dequant_mx: out_dev is NULL or not aligned to its type");
+  hipError_t err = ce_mx_dequant((const uint8_t*)q_dev, scale_dev, fmt, n_rows, k, out_dev, out_dtype, (hipStream_t)stream);
+  if (err != hipSuccess) return fail("dequant_mx(%ld,%d) failed: %s", n_rows, k, hipGetErrorString(err));
+  return 0;
+}
+
+int clipenc_op_norm_quant_mx(const void* in_dev, int in_dtype, long n_rows, int k, long ld_in, const void* resid_dev, long ld_resid, int norm,
+                             const float* gamma_dev, const float* beta_dev, float eps, int fmt, void* h_out_dev, void* out_dev,
+                             void* scale_dev, void* stream) {
+  if (int rc = mx_check_rows("norm_quant_mx", in_dev, in_dtype, n_rows, k, ld_in)) return rc;
+  if (k > MX_NORM_MAX_K) return fail("norm_quant_mx: k = %d (at most %d)", k, MX_NORM_MAX_K);
+  if (norm != CLIPENC_NORM_RMS && norm != CLIPENC_NORM_LAYER) return fail("norm_quant_mx: norm = %d (CLIPENC_NORM_*)", norm);
+  if (fmt < CLIPENC_MX_E2M1 || fmt > CLIPENC_ROW_E4M3) return fail("norm_quant_mx: fmt = %d", fmt);
+  if (!(eps >= 0.0f)) return fail("norm_quant_mx: eps = %g", (double)eps);
+  if ((resid_dev == nullptr) != (h_out_dev == nullptr)) return fail("norm_quant_mx: resid_dev and h_out_dev come together");
+  if (n_rows == 0) return 0;
+  if (resid_dev) {
+    if (int rc = mx_check_rows("norm_quant_mx (resid)", resid_dev, in_dtype, n_rows, k, ld_resid)) return rc;
+    if (!aligned_to(h_out_dev, dt_size(in_dtype))) return fail("norm_quant_mx: h_out_dev is not aligned to its type");
+    if ((h_out_dev == in_dev && ld_in != k) || (h_out_dev == resid_dev && ld_resid != k))
+      return fail("norm_quant_mx: h_out_dev may be an input only where its rows are k elements apart");
+  }
+  if (!gamma_dev || !aligned_to(gamma_dev, 4) || !aligned_to(beta_dev, 4)) return fail("norm_quant_mx: gamma_dev is NULL, or gamma / beta not 4-byte aligned");
+  if (int rc = mx_check_q("norm_quant_mx", out_dev, scale_dev)) return rc;
+  MxNormParams p{};
+  p.x = in_dev; p.ld_x = ld_in; p.resid = resid_dev; p.ld_r = ld_resid; p.gamma = gamma_dev; p.beta = beta_dev; p.h = h_out_dev;
+  p.q = (uint8_t*)out_dev; p.scale = scale_dev; p.n_rows = n_rows; p.k = k; p.kp = mx_kp(k); p.norm = norm; p.fmt = fmt; p.eps = eps;
+  hipError_t err = ce_mx_norm(p, in_dtype, (hipStream_t)stream);
+  if (err != hipSuccess) return fail("norm_quant_mx(%ld,%d) failed: %s", n_rows, k, hipGetErrorString(err));
+  return 0;
+}
+
+int clipenc_op_gemm_mx(const void* a_dev, const void* a_scale_dev, int a_fmt, const void* w_dev, const void* w_scale_dev, int m, int n, int k,
+                       const float* bias_dev, int act, const void* resid_dev, void* out_dev, int out_dtype, void* stream) {
+  if (int rc = mx_check_product("gemm_mx", w_dev, w_scale_dev, m, n, k, bias_dev, act, resid_dev, out_dev, out_dtype)) return rc;
+  if (a_fmt != CLIPENC_MX_E2M1 && a_fmt != CLIPENC_MX_E4M3) return fail("gemm_mx: a_fmt = %d (CLIPENC_MX_E2M1 or CLIPENC_MX_E4M3)", a_fmt);
+  if (m == 0 || n == 0) return 0;
+  if (int rc = mx_check_q("gemm_mx", a_dev, a_scale_dev)) return rc;
+  MxGemmParams p{};
+  p.a = (const uint8_t*)a_dev; p.a_scale = (const uint8_t*)a_scale_dev; p.w = (const uint8_t*)w_dev; p.w_scale = (const uint8_t*)w_scale_dev;
+  p.M = m; p.N = n; p.nk = mx_kp(k) / 128; p.bias = bias_dev; p.resid = resid_dev; p.out = out_dev; p.act = act; p.out_dtype = out_dtype;
+  hipError_t err = ce_mx_gemm(p, a_fmt, (hipStream_t)stream);
+  if (err != hipSuccess) return fail("gemm_mx(%d,%d,%d) failed: %s", m, n, k, hipGetErrorString(err));
+  return 0;
+}
+
+size_t clipenc_op_linear_mx_ws_bytes(int m, int k, int x_fmt) {
+  if (m < 1 || k < 1 || k > MX_MAX_K || (x_fmt != CLIPENC_MX_E2M1 && x_fmt != CLIPENC_MX_E4M3)) return 0;
+  return (size_t)m * (mx_row_bytes(k, x_fmt) + (size_t)mx_kp(k) / 32);
+}
+
+int clipenc_op_linear_mx(const void* in_dev, int in_dtype, long ld_in, int x_fmt, const void* w_dev, const void* w_scale_dev, int m, int n,
+                         int k, const float* bias_dev, int act, const void* resid_dev, void* out_dev, int out_dtype, void* ws_dev,
+                         size_t ws_bytes, void* stream) {
+  if (int rc = mx_check_product("linear_mx", w_dev, w_scale_dev, m, n, k, bias_dev, act, resid_dev, out_dev, out_dtype)) return rc;
+  if (int rc = mx_check_rows("linear_mx", in_dev, in_dtype, m, k, ld_in)) return rc;
+  if (x_fmt != CLIPENC_MX_E2M1 && x_fmt != CLIPENC_MX_E4M3) return fail("linear_mx: x_fmt = %d (CLIPENC_MX_E2M1 or CLIPENC_MX_E4M3)", x_fmt);
+  if (m == 0 || n == 0) return 0;
+  const size_t need = clipenc_op_linear_mx_ws_bytes(m, k, x_fmt);
+  if (need && (!ws_dev || ws_bytes < need || !aligned_to(ws_dev, 16))) return fail("linear_mx: scratch of %zu bytes, 16-byte aligned, is needed: %zu given", need, ws_dev ? ws_bytes : (size_t)0);
+  uint8_t* q = (uint8_t*)ws_dev;
+  uint8_t* s = q + (size_t)m * mx_row_bytes(k, x_fmt);
+  if (int rc = clipenc_op_quant_mx(in_dev, in_dtype, m, k, ld_in, x_fmt, q, s, stream)) return rc;
+  return clipenc_op_gemm_mx(q, s, x_fmt, w_dev, w_scale_dev, m, n, k, bias_dev, act, resid_dev, out_dev, out_dtype, stream);
 }
 
 int clipenc_op_quant_block_fp8(const void* in_dev, int n_rows, int k, void* out8_dev, void* exp_dev, float* stats_dev,

@@ -347,6 +347,48 @@ int clipenc_op_gemm_fp8_lnf(const void* a8_dev, const void* exp_dev, const void*
 int clipenc_op_gemm_fp8_resid_q(const void* a8_dev, const void* w8_dev, int m, int n, int k, const float* scale_w_dev,
                                 const float* bias_dev, void* x_inout_dev, void* out8_dev, void* exp_dev, float* stats_dev,
                                 int stats_ld, void* stream);
+/* ---- Microscaled (OCP MX) rows: e2m1 (4-bit) or e4m3 elements, one power-of-two scale per 32 columns; inference operators.
+ * A quantised matrix of n_rows x k has rows of kp = k rounded up to 128 columns, the added ones zero:
+ *   elements  CLIPENC_MX_E2M1: kp / 2 bytes a row, the lower column in the low half of a byte;  CLIPENC_MX_E4M3: kp bytes a row
+ *   scales    kp / 32 bytes a row: X + 127 of the block's scale 2^X, X = clamp(floor(log2 max|v|) - emax, -127, 127), emax = 2 / 8;
+ *             0xff: the block held an infinity or a NaN and is NaN
+ * elements are v / 2^X rounded to nearest (ties to even), at most 6 / 448.  CLIPENC_ROW_E4M3: kp e4m3 bytes a row and ONE float scale a
+ * row, max|v| / 448 (0 for a zero row, NaN for one that is not finite): what clipenc_op_gemm_fp8 takes as scale_a where k % 256 == 0.
+ * All matrices are row-major; elements 16-byte aligned, scale bytes 4-byte aligned, values aligned to their type only; 1 <= k <= 2^20.
+ * Nothing is read or written behind the last row; zero rows (n_rows, m or n = 0) are a call that does nothing.  Every call is
+ * deterministic, needs no scratch but what it names, and may be captured into a graph. */
+#define CLIPENC_DT_F32 2
+#define CLIPENC_MX_E2M1 0
+#define CLIPENC_MX_E4M3 1
+#define CLIPENC_ROW_E4M3 2
+#define CLIPENC_NORM_RMS 0
+#define CLIPENC_NORM_LAYER 1
+/* Rows of k values, ld_in elements apart (>= k), of in_dtype (CLIPENC_DT_*) -> fmt CLIPENC_MX_E2M1 / CLIPENC_MX_E4M3. */
+int clipenc_op_quant_mx(const void* in_dev, int in_dtype, long n_rows, int k, long ld_in, int fmt, void* out_dev, void* scale_dev,
+                        void* stream);
+/* The values a quantised matrix stands for, [n_rows][k] of out_dtype (any of the three formats). */
+int clipenc_op_dequant_mx(const void* q_dev, const void* scale_dev, int fmt, long n_rows, int k, void* out_dev, int out_dtype,
+                          void* stream);
+/* A norm with the residual's addition that ends in quantised rows:
+ *   h = in + resid, rounded to in_dtype, as it is stored in h_out_dev [n_rows][k] (resid_dev and h_out_dev both NULL: h = in)
+ *   y = h * gamma / sqrt(mean(h^2) + eps) + beta             norm = CLIPENC_NORM_RMS
+ *       (h - mean(h)) * gamma / sqrt(var(h) + eps) + beta           CLIPENC_NORM_LAYER       (beta_dev may be NULL)
+ * and y in fmt (any of the three).  gamma / beta: float [k]; k <= 16384; ld_in / ld_resid in elements; h_out_dev may be in_dev or
+ * resid_dev where that one's rows are k elements apart.  Sums and the row's factor are held in 64 bits. */
+int clipenc_op_norm_quant_mx(const void* in_dev, int in_dtype, long n_rows, int k, long ld_in, const void* resid_dev, long ld_resid, int norm,
+                             const float* gamma_dev, const float* beta_dev, float eps, int fmt, void* h_out_dev, void* out_dev,
+                             void* scale_dev, void* stream);
+/* out[m][n] = act(A . W^T + bias[n]) + resid[m][n]:  A [m] rows of a_fmt (CLIPENC_MX_E2M1 / _E4M3), W [n] rows of CLIPENC_MX_E2M1, both of k
+ * columns; products and sums in fp32, one rounding to out_dtype.  bias_dev (float [n]) and resid_dev ([m][n] of out_dtype, may be
+ * out_dev) may be NULL; act: -1 none, CLIPENC_ACT_*; not both act and resid. */
+int clipenc_op_gemm_mx(const void* a_dev, const void* a_scale_dev, int a_fmt, const void* w_dev, const void* w_scale_dev, int m, int n, int k,
+                       const float* bias_dev, int act, const void* resid_dev, void* out_dev, int out_dtype, void* stream);
+/* The same from values: A = quantised `in` (as clipenc_op_quant_mx to x_fmt), in one call.  ws_dev: 16-byte aligned scratch of
+ * clipenc_op_linear_mx_ws_bytes(m, k, x_fmt) bytes (0 where the product takes the values as they are: ws_dev may be NULL then). */
+size_t clipenc_op_linear_mx_ws_bytes(int m, int k, int x_fmt);
+int clipenc_op_linear_mx(const void* in_dev, int in_dtype, long ld_in, int x_fmt, const void* w_dev, const void* w_scale_dev, int m, int n,
+                         int k, const float* bias_dev, int act, const void* resid_dev, void* out_dev, int out_dtype, void* ws_dev,
+                         size_t ws_bytes, void* stream);
 /* qkv bf16 [n_crops*n_tok][3*width] -> out bf16 [n_crops*n_tok][width]; head dim 64, n_tok <= 640 */
 int clipenc_op_attention(const void* qkv_dev, void* out_dev, int n_crops, int n_tok, int width, int heads,
                          void* stream);
