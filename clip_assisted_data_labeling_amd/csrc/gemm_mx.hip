@@ -13,12 +13,18 @@
 // for 16-bit results.  An fp32 result gets the sum in two BANDS of e4m3 codes, exponent fields 8 .. 15 and 0 .. 7: a band's products span
 // at most 14 bits (2^-3 .. 2^11, 2^-10 .. 2^3), so nothing is cut, at two MFMAs a fragment pair.
 //
-// Tiles of BM x BN, WM x WN waves.  K goes by stages of 256 columns: 128-byte rows of W (and of an e2m1 A; an e4m3 A has two such
-// halves a stage), brought in by LDS-DMA in pieces of 8 rows x 128 bytes, two stages of LDS in turn: stage s + 1 lands while stage s is
-// multiplied.  The 16-byte chunk c of tile row r lies at chunk c ^ ((r >> 1) & 7) of its row, by the choice of the DMA's source
-// addresses, so that 16 lanes reading one chunk column of 16 rows meet no bank twice.  Scales come by periods of 512 columns: a
-// thread brings the four words of a row, turns the 4 x 4 bytes round -- word g: the scales of block g in the period's four K steps --
-// and a lane reads ONE word per 16 rows and period, with the K step as opsel.
+// Persistent tiles of BM x BN, WM x WN waves.  LDS holds two stages of 128-byte rows of A (256 columns of e2m1, 128 of e4m3) and two of W
+// (256 columns), brought in by LDS-DMA in pieces of 8 rows x 128 bytes.  The walk is one sequence of stages over all of a workgroup's
+// tiles: a stage's last fragments are in registers before its end, so the barrier there frees its buffer, the stage after next is asked
+// for -- of this tile or the next one --, the next stage's first fragments are read under the last products, and a finished tile's
+// results leave straight from the registers while the next tile's rows arrive.  The 16-byte chunk c of tile row r lies at chunk
+// c ^ ((r >> 1) & 7) of its row, by the choice of the DMA's source addresses, so that 16 lanes reading one chunk column of 16 rows meet no
+// bank twice.  K steps are counted in pairs; an odd number of them is led by an empty one, which e4m3 rows skip and e2m1 rows multiply
+// with both scales at 2^-127: products below 2^-240, zeros in fp32.
+// Scales come by periods of 512 columns, the four words of a row turned round -- word g: the scales of block g in the period's four K
+// steps -- so that a lane holds the scales of 16 rows and a period in ONE word.
+#include <type_traits>
+
 #include "common.h"
 #include "mx.h"
 
@@ -30,17 +36,40 @@ typedef __attribute__((ext_vector_type(4))) int i32x4_t;
 typedef __attribute__((ext_vector_type(8))) int i32x8_t;
 typedef __attribute__((ext_vector_type(4))) uint32_t u32x4_t;
 
-__device__ __forceinline__ float activate(float u, int act) {
-  if (act == CE_ACT_QUICK_GELU) return u * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-2.4554669595930156f * u));
-  if (act == CE_ACT_GELU_ERF) return ce_gelu_erf(u);
-  return u;
+// N vectors at once, stage by stage: the exp2s and rcps stand apart from their consumers, one branch for all
+template <int N>
+__device__ __forceinline__ void activate(f32x4_t (&v)[N], int act) {
+  if (act == CE_ACT_QUICK_GELU) {
+    f32x4_t t[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) t[j][e] = __builtin_amdgcn_exp2f(v[j][e] * -2.4554669595930156f);
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) t[j][e] = __builtin_amdgcn_rcpf(1.0f + t[j][e]);
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] *= t[j];
+  } else if (act == CE_ACT_GELU_ERF) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = ce_gelu_erf4(v[j]);
+  }
 }
 
-// 64 lanes x 16 bytes from base + offset (per lane) to the 1 KiB of LDS at lds_addr.  Inline asm: behind the builtin every later
-// LDS read would first wait for all pieces in flight.  m0 is written; nothing else here uses it.
+// 64 lanes x 16 (4) bytes from base + offset (per lane) to the 1 KiB (256 bytes) of LDS at lds_addr.  Inline asm: behind the builtin every
+// later LDS read would first wait for all pieces in flight.  m0 is written; nothing else here uses it.
+__device__ __forceinline__ const uint8_t* uniform(const uint8_t* p) {
+  const uint64_t b = (uint64_t)p;
+  return (const uint8_t*)((uint64_t)__builtin_amdgcn_readfirstlane((unsigned)(b >> 32)) << 32 | (unsigned)__builtin_amdgcn_readfirstlane((unsigned)b));
+}
 __device__ __forceinline__ void dma16(const uint8_t* base, unsigned off, unsigned lds_addr) {
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(base), "s"(lds_addr) : "memory");
 }
+__device__ __forceinline__ void dma4(const uint8_t* base, unsigned off, unsigned lds_addr) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" : : "v"(off), "s"(base), "s"(lds_addr) : "memory");
+}
+#define WAIT_LDS() asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory")
 #define WAIT_ALL() asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" : : : "memory")
 #define BARRIER() asm volatile("s_barrier" : : : "memory")
 
@@ -58,33 +87,41 @@ __device__ __forceinline__ void store_elem(void* p, size_t i, int dtype, float v
 // rows of `out` start at any element: no more than its own alignment is promised
 struct __attribute__((packed, aligned(2))) Pack16 { u32x4_t v; };
 struct __attribute__((packed, aligned(4))) Pack32 { u32x4_t v; };
+typedef uint32_t stream16_t __attribute__((ext_vector_type(4), aligned(2)));
 
-// Columns n .. n + 7 of row m, all of them inside: v (+ resid) to 16 bits
-__device__ __forceinline__ void store8_16bit(const MxGemmParams& p, size_t at, const float (&v)[8]) {
-  float r[8];
+// 8 values + 8 of 16 bits (r, if with), rounded once to 16 bits
+__device__ __forceinline__ u32x4_t to_16bit(f32x4_t a, f32x4_t b, u32x4_t r, bool with, int dtype) {
+  u32x4_t o;
+  if (dtype == MX_DT_BF16) {
+    if (with) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) r[i] = v[i];
-  Pack16 o;
-  if (p.out_dtype == MX_DT_BF16) {
-    if (p.resid) {
-      const u32x4_t s = ((const Pack16*)((const bf16_t*)p.resid + at))->v;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) { r[2 * i] += __uint_as_float(s[i] << 16); r[2 * i + 1] += __uint_as_float(s[i] & 0xffff0000u); }
+      for (int i = 0; i < 2; ++i) {
+        a[2 * i] += __uint_as_float(r[i] << 16); a[2 * i + 1] += __uint_as_float(r[i] & 0xffff0000u);
+        b[2 * i] += __uint_as_float(r[i + 2] << 16); b[2 * i + 1] += __uint_as_float(r[i + 2] & 0xffff0000u);
+      }
     }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o.v[i] = pack_bf16x2(r[2 * i], r[2 * i + 1]);
+    o[0] = pack_bf16x2(a[0], a[1]); o[1] = pack_bf16x2(a[2], a[3]); o[2] = pack_bf16x2(b[0], b[1]); o[3] = pack_bf16x2(b[2], b[3]);
   } else {
+    const f16x8_t s = __builtin_bit_cast(f16x8_t, r);
     f16x8_t h;
-    if (p.resid) {
-      const f16x8_t s = __builtin_bit_cast(f16x8_t, ((const Pack16*)((const _Float16*)p.resid + at))->v);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) r[i] += (float)s[i];
+    for (int i = 0; i < 4; ++i) {
+      h[i] = (_Float16)(with ? a[i] + (float)s[i] : a[i]);
+      h[i + 4] = (_Float16)(with ? b[i] + (float)s[i + 4] : b[i]);
     }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) h[i] = (_Float16)r[i];
-    o.v = __builtin_bit_cast(u32x4_t, h);
+    o = __builtin_bit_cast(u32x4_t, h);
   }
-  *(Pack16*)((uint16_t*)p.out + at) = o;
+  return o;
+}
+// The fragments of two neighbouring column groups (a: columns 4 g .. 4 g + 3 of the first, b: of the second) -> eight neighbouring columns
+// a lane, from column 16 (g & 1) + 8 (g >> 1) of the pair: odd rows of 16 lanes change places between the two registers.
+__device__ __forceinline__ void pair_columns(f32x4_t& a, f32x4_t& b) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(a[e]), __float_as_uint(b[e]), false, false);
+    a[e] = __uint_as_float(s[0]);
+    b[e] = __uint_as_float(s[1]);
+  }
 }
 
 // the e4m3 codes with exponent fields 8 .. 15 (bit 6 of the byte), zeros in the place of the others
@@ -98,247 +135,348 @@ __device__ __forceinline__ i32x8_t high_band(i32x8_t v) {
   return r;
 }
 
-template <int AF, int BM, int BN, int WM, int WN>
+template <int CTRL>   // CTRL: quad_perm
+__device__ __forceinline__ uint32_t dpp_quad(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true); }
+
+template <int I, int N, typename F>
+__device__ __forceinline__ void for_each_int(F&& f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>{});
+    for_each_int<I + 1, N>(f);
+  }
+}
+
+template <int AF, int BM_, int BN_, int WM_, int WN_>
 struct Tile {
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
   static constexpr int NW = WM * WN, THREADS = NW * 64;
   static constexpr int FM = BM / WM / 16, FN = BN / WN / 16;       // 16 x 16 fragments of a wave
-  static constexpr int A_HALF = BM * 128, A_BYTES = A_HALF * (AF != A_E2M1 ? 2 : 1), W_BYTES = BN * 128;
-  static constexpr int STAGE = A_BYTES + W_BYTES;
-  static constexpr int A_PIECES = A_BYTES / 1024, PIECES = STAGE / 1024, PER_WAVE = PIECES / NW;
-  static constexpr int SC_ROWS = BM + BN, SC_BYTES = SC_ROWS * 16, SC_OFF = 2 * STAGE;
-  static constexpr int SC_PER = (SC_ROWS + THREADS - 1) / THREADS;
-  static constexpr int LDS = 2 * STAGE + 2 * SC_BYTES;
-  static constexpr int IMG = 4096;                                  // a wave's 16 x 64 fp32 results on their way out
-  static_assert(PIECES % NW == 0 && FM >= 1 && FN >= 1 && NW * IMG <= 2 * STAGE && LDS <= 163840, "tile");
+  static constexpr int STEPS = AF == A_E2M1 ? 2 : 1;               // K steps of a stage of A
+  static constexpr int A_BYTES = BM * 128, W_BYTES = BN * 128;
+  static constexpr int A_PER = BM / 8 / NW, W_PER = BN / 8 / NW;   // DMA pieces a wave
+  static constexpr int W_OFF = 2 * A_BYTES, SC_OFF = W_OFF + 2 * W_BYTES;
+  static constexpr int SC_ROWS = BM + BN, SC_BYTES = SC_ROWS * 16, SC_PER = SC_ROWS * 4 / THREADS;
+  static constexpr int RAW_OFF = SC_OFF + 2 * SC_BYTES, BIAS_OFF = RAW_OFF + SC_BYTES, LDS = BIAS_OFF + 2 * BN * 4;
+  static constexpr int STORES = FM * FN / 2;                       // of a wave's whole 16-bit tile, 16 bytes a lane each
+  static_assert(A_PER >= W_PER && FM >= 2 && FN % 2 == 0 && A_PER * NW * 8 == BM && W_PER * NW * 8 == BN && NW % 2 == 0, "pieces");
+  static_assert(SC_PER * THREADS == SC_ROWS * 4 && BM % (THREADS / 4) == 0 && BN % 64 == 0 && BN <= THREADS, "scales, bias");
+  static_assert(LDS <= 163840, "LDS");
 };
 
 template <int AF, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(WM * WN * 64, WM * WN == 8 ? 2 : 2) void mx_gemm_kernel(const MxGemmParams p) {
+__global__ __launch_bounds__(WM * WN * 64, 2) void mx_gemm_kernel(const MxGemmParams p) {
   using T = Tile<AF, BM, BN, WM, WN>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = w / WN, wn = w % WN;
   const int r16 = lane & 15, g = lane >> 4;
-
-  // neighbouring workgroups of one XCD (blockIdx mod 8) walk neighbouring tiles, 8 row tiles deep
-  const int tiles_m = (p.M + BM - 1) / BM, tiles_n = (p.N + BN - 1) / BN;
-  const int nwg = tiles_m * tiles_n;
-  const int q = nwg >> 3, rem = nwg & 7, xcd = blockIdx.x & 7, pos = blockIdx.x >> 3;
-  const int bid = (xcd < rem ? xcd * (q + 1) : rem * (q + 1) + (xcd - rem) * q) + pos;
-  constexpr int GM = 8;
-  const int first = bid / (GM * tiles_n) * GM, depth = min(tiles_m - first, GM), in_group = bid % (GM * tiles_n);
-  const int m0 = (first + in_group % depth) * BM, n0 = in_group / depth * BN;
-
-  const int a_ld = p.nk * (AF != A_E2M1 ? 128 : 64), w_ld = p.nk * 64;
-  const uint8_t* a_tile = p.a + (size_t)m0 * a_ld;
-  const uint8_t* w_tile = p.w + (size_t)n0 * w_ld;
   const unsigned lds0 = __builtin_amdgcn_readfirstlane((unsigned)(size_t)(__attribute__((address_space(3))) char*)smem);
 
-  // This wave's pieces: piece w + i NW.  The lane's source: row (lane >> 3) of the piece, chunk (lane & 7) ^ swizzle; rows behind the
-  // matrix repeat its last one (their results are not stored).  half_off: what to take off the columns when a stage's second K step
-  // lies behind the row's end (those bytes are not multiplied).
-  unsigned src[T::PER_WAVE];
-  const int lr = lane >> 3;
+  // tile i of the walk: neighbouring workgroups of one XCD (i mod 8) walk neighbouring tiles, 8 row tiles deep
+  const int tiles_m = (p.M + BM - 1) / BM, tiles_n = (p.N + BN - 1) / BN;
+  const int nwg = tiles_m * tiles_n;
+  auto tile_at = [&](int i, int& m0, int& n0) {
+    const int q = nwg >> 3, rem = nwg & 7, xcd = i & 7, pos = i >> 3;
+    const int bid = (xcd < rem ? xcd * (q + 1) : rem * (q + 1) + (xcd - rem) * q) + pos;
+    constexpr int GM = 8;
+    const int first = bid / (GM * tiles_n) * GM, depth = min(tiles_m - first, GM), in_group = bid % (GM * tiles_n);
+    m0 = (first + in_group % depth) * BM;
+    n0 = in_group / depth * BN;
+  };
+
+  const int odd = p.nk & 1, steps = p.nk + odd;                     // K steps counted with the empty one in front
+  const unsigned a_ld = (unsigned)p.nk * (AF == A_E2M1 ? 64u : 128u), w_ld = (unsigned)p.nk * 64u;
+
+  // DMA of a piece: the lane's row is lane >> 3 of its 8, its chunk (lane & 7) ^ swizzle -- the same of all of a wave's pieces, whose
+  // blocks of 8 rows are w, w + NW, ...: of w's parity.  Rows behind the matrix repeat its last one (their results are not stored).
+  // Where the first step is the empty one (lead_in), its half of the row is read from the second one's columns.
+  const int lr = lane >> 3, chunk = (lane & 7) ^ ((w & 1) << 2 | lr >> 1);
+  const unsigned a_off = (unsigned)(w * 8 + lr) * a_ld + (unsigned)(chunk * 16), w_off = (unsigned)(w * 8 + lr) * w_ld + (unsigned)(chunk * 16);
+  const unsigned lead = chunk < 4 ? 64u : 0u, low = (unsigned)(chunk * 16);
+  const uint64_t a_hop = (uint64_t)(T::NW * 8) * a_ld, w_hop = (uint64_t)(T::NW * 8) * w_ld;
+  auto issue = [&](const uint8_t* base, unsigned off, uint64_t hop, unsigned last, bool whole, bool lead_in, auto per_, unsigned dst) {
+    constexpr int PER = decltype(per_)::value;       // last: the offset of the last row
+    const unsigned plus = lead_in ? lead : 0u;
+    if (whole) {
 #pragma unroll
-  for (int i = 0; i < T::PER_WAVE; ++i) {
-    const int piece = w + i * T::NW;
-    const bool is_a = piece < T::A_PIECES;
-    const int half = AF != A_E2M1 && is_a ? piece / (BM / 8) : 0;
-    const int block = is_a ? piece - half * (BM / 8) : piece - T::A_PIECES;
-    const int row = block * 8 + lr;
-    const int chunk = (lane & 7) ^ ((row >> 1) & 7);
-    const int limit = (is_a ? p.M - m0 : p.N - n0) - 1;
-    src[i] = (unsigned)min(row, limit) * (unsigned)(is_a ? a_ld : w_ld) + (unsigned)(chunk * 16 + half * 128);
-  }
-  const int chunk_of = (lane & 7) ^ ((((w & 1) << 2) | (lr >> 1)) & 7);   // the same of all of the wave's pieces: their parity is w's
-  auto issue = [&](int st, int buf) {
-    const int ks = 2 * st;
-    const bool half = ks + 1 >= p.nk;                                     // the stage's second K step lies behind the end
+      for (int i = 0; i < PER; ++i) dma16(base + i * hop, off + plus, dst + (unsigned)(i * T::NW * 1024));
+    } else {
 #pragma unroll
-    for (int i = 0; i < T::PER_WAVE; ++i) {
-      const int piece = w + i * T::NW;
-      const bool is_a = piece < T::A_PIECES;
-      unsigned off = src[i];
-      if (half) {
-        if (AF != A_E2M1 && is_a) { if (piece >= BM / 8) off -= 128; }
-        else if (chunk_of >= 4) off -= 64;
-      }
-      const uint8_t* base = is_a ? a_tile + (size_t)ks * (AF != A_E2M1 ? 128 : 64) : w_tile + (size_t)ks * 64;
-      dma16(base, off, lds0 + (unsigned)(buf * T::STAGE + piece * 1024));
+      for (int i = 0; i < PER; ++i) dma16(base, min(off - low + i * (unsigned)hop, last) + low + plus, dst + (unsigned)(i * T::NW * 1024));
     }
   };
 
-  // scales: thread t brings the period's four words of rows t, t + THREADS, ...  (rows 0 .. BM - 1: A, then W)
-  u32x4_t sc[T::SC_PER];
-  auto scales_load = [&](int period) {
+  // Scales: four neighbouring lanes bring the period's four words of a row (16 rows an instruction: a lane a word of 64 rows would
+  // touch four times the lines), rows of A first, then those of W; words before a row's first and behind its last one repeat a
+  // neighbour.  They land as they are; each thread then turns the 4 x 4 bytes round with its neighbours -- words that its own wave has
+  // brought -- and leaves its word where the fragments' lanes read it.
+  const unsigned s_ld = (unsigned)p.nk * 4u;
+  const int periods = (steps + 3) >> 2;
+  auto issue_scales = [&](const uint8_t* a_at, const uint8_t* w_at, int a_rows, int w_rows, int period) {
+    // (a_at, w_at: where the period's words of the tile's first rows would begin)
+    unsigned j = (unsigned)(tid & 3) * 4u;
+    if (period == 0 && odd) j = max(j, 4u);
+    if (period == periods - 1 && (steps & 2)) j = min(j, 4u);
 #pragma unroll
     for (int i = 0; i < T::SC_PER; ++i) {
-      const int row = tid + i * T::THREADS;
-      const bool is_a = row < BM;
-      const size_t at = is_a ? (size_t)min(m0 + row, p.M - 1) : (size_t)min(n0 + row - BM, p.N - 1);
-      const uint32_t* s = (const uint32_t*)(is_a ? p.a_scale : p.w_scale) + at * p.nk;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) sc[i][j] = s[min(period * 4 + j, p.nk - 1)];
+      const bool is_a = i * (T::THREADS / 4) < BM;
+      const int row = i * (T::THREADS / 4) + (tid >> 2) - (is_a ? 0 : BM);
+      dma4(is_a ? a_at : w_at, (unsigned)min(row, (is_a ? a_rows : w_rows) - 1) * s_ld + j, lds0 + (unsigned)(T::RAW_OFF + (i * T::THREADS + w * 64) * 4));
     }
   };
-  auto scales_store = [&](int buf) {
+  const uint32_t sc_sel = 0x01010101u * (uint32_t)(tid & 3) + 0x00000400u;      // bytes (own, own + 4) of a register pair
+  auto turn_scales = [&](int period, int buf) {
+    const uint32_t keep = AF == A_E2M1 && odd && period == 0 && (tid & 3) == 0 ? 0u : 0xffffffffu;   // the empty step's word
 #pragma unroll
     for (int i = 0; i < T::SC_PER; ++i) {
-      const uint32_t lo01 = __builtin_amdgcn_perm(sc[i][1], sc[i][0], 0x05010400u), hi01 = __builtin_amdgcn_perm(sc[i][1], sc[i][0], 0x07030602u);
-      const uint32_t lo23 = __builtin_amdgcn_perm(sc[i][3], sc[i][2], 0x05010400u), hi23 = __builtin_amdgcn_perm(sc[i][3], sc[i][2], 0x07030602u);
-      u32x4_t o;
-      o[0] = __builtin_amdgcn_perm(lo23, lo01, 0x05040100u);
-      o[1] = __builtin_amdgcn_perm(lo23, lo01, 0x07060302u);
-      o[2] = __builtin_amdgcn_perm(hi23, hi01, 0x05040100u);
-      o[3] = __builtin_amdgcn_perm(hi23, hi01, 0x07060302u);
-      if (T::SC_ROWS % T::THREADS == 0 || tid + i * T::THREADS < T::SC_ROWS)
-        *(u32x4_t*)(smem + T::SC_OFF + buf * T::SC_BYTES + (tid + i * T::THREADS) * 16) = o;
+      const int at = (i * T::THREADS + tid) * 4;
+      const uint32_t s = *(volatile const uint32_t*)(smem + T::RAW_OFF + at) & keep;
+      const uint32_t w0 = dpp_quad<0x00>(s), w1 = dpp_quad<0x55>(s), w2 = dpp_quad<0xAA>(s), w3 = dpp_quad<0xFF>(s);
+      const uint32_t lo = __builtin_amdgcn_perm(w1, w0, sc_sel), hi = __builtin_amdgcn_perm(w3, w2, sc_sel);
+      *(uint32_t*)(smem + T::SC_OFF + buf * T::SC_BYTES + at) = __builtin_amdgcn_perm(hi, lo, 0x05040100u);
     }
   };
 
   f32x4_t acc[T::FM][T::FN];
-#pragma unroll
-  for (int i = 0; i < T::FM; ++i)
-#pragma unroll
-    for (int j = 0; j < T::FN; ++j) acc[i][j] = f32x4_t{0, 0, 0, 0};
-
   const int rd = (r16 >> 3) * 1024 + (r16 & 7) * 128 + ((g ^ ((r16 >> 1) & 7)) << 4);   // chunk g of row r16; chunk g + 4: ^ 64
-  uint32_t sa[T::FM], sw[T::FN];
-  auto scales_read = [&](int buf) {
-    const char* s = smem + T::SC_OFF + buf * T::SC_BYTES + r16 * 16 + g * 4;
-#pragma unroll
-    for (int i = 0; i < T::FM; ++i) sa[i] = *(const uint32_t*)(s + (wm * T::FM + i) * 256);
-#pragma unroll
-    for (int j = 0; j < T::FN; ++j) sw[j] = *(const uint32_t*)(s + (T::FM * WM + wn * T::FN + j) * 256);
+  // Fragments of a stage whose first K step is number `in_period` (0 .. 3) of its period
+  auto load_w = [&](int wbuf, int in_period, int step, int j) {
+    const int at = AF == A_E2M1 ? rd : rd ^ ((in_period & 1) * 64);
+    const i32x4_t v = *(const i32x4_t*)(smem + T::W_OFF + wbuf * T::W_BYTES + (wn * T::FN + j) * 2048 + (at ^ (step * 64)));
+    return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1);
   };
-#define MX_STEP(BUF, KS, OP)                                                                                                    \
-  {                                                                                                                              \
-    const char* at = smem + (BUF) * T::STAGE;                                                                                    \
-    i32x8_t wf[T::FN];                                                                                                           \
-    _Pragma("unroll") for (int j = 0; j < T::FN; ++j) {                                                                          \
-      const i32x4_t v = *(const i32x4_t*)(at + T::A_BYTES + (wn * T::FN + j) * 2048 + (rd ^ ((KS) * 64)));                       \
-      wf[j] = __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1);                                                         \
-    }                                                                                                                            \
-    _Pragma("unroll") for (int i = 0; i < T::FM; ++i) {                                                                          \
-      i32x8_t af;                                                                                                                \
-      if constexpr (AF != A_E2M1) {                                                                                             \
-        const char* s = at + (KS) * T::A_HALF + (wm * T::FM + i) * 2048;                                                         \
-        const i32x4_t lo = *(const i32x4_t*)(s + rd), hi = *(const i32x4_t*)(s + (rd ^ 64));                                     \
-        af = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);                                                            \
-      } else {                                                                                                                   \
-        const i32x4_t v = *(const i32x4_t*)(at + (wm * T::FM + i) * 2048 + (rd ^ ((KS) * 64)));                                  \
-        af = __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1);                                                          \
-      }                                                                                                                          \
-      if constexpr (AF == A_E4M3_BANDS) {                                                                                        \
-        const i32x8_t high = high_band(af);                                                                                      \
-        af ^= high;                                                                                                              \
-        _Pragma("unroll") for (int j = 0; j < T::FN; ++j)                                                                        \
-          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[j], high, acc[i][j], 4, 0, OP, (int)sw[j], OP,         \
-                                                                       (int)sa[i]);                                              \
-      }                                                                                                                          \
-      _Pragma("unroll") for (int j = 0; j < T::FN; ++j)                                                                          \
-        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[j], af, acc[i][j], 4, AF != A_E2M1 ? 0 : 4, OP,          \
-                                                                     (int)sw[j], OP, (int)sa[i]);                                \
-    }                                                                                                                            \
-  }
+  auto load_a = [&](int abuf, int step, int i) {
+    const char* at = smem + abuf * T::A_BYTES + (wm * T::FM + i) * 2048;
+    if constexpr (AF != A_E2M1) {
+      const i32x4_t lo = *(const i32x4_t*)(at + rd), hi = *(const i32x4_t*)(at + (rd ^ 64));
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    } else {
+      const i32x4_t v = *(const i32x4_t*)(at + (rd ^ (step * 64)));
+      return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1);
+    }
+  };
+  auto load_scale = [&](int sbuf, int in_period, int row16) -> uint32_t {   // the stage's one or two bytes of the lane's word
+    const char* at = smem + T::SC_OFF + sbuf * T::SC_BYTES + r16 * 16 + g * 4 + row16 * 256 + in_period;
+    return T::STEPS == 2 ? (uint32_t)*(const uint16_t*)at : (uint32_t)*(const uint8_t*)at;
+  };
+  constexpr int FM = T::FM, FN = T::FN, N = T::STEPS * FM;          // N row fragments a stage
 
-  const int stages = (p.nk + 1) >> 1;
-  scales_load(0);
-  issue(0, 0);
+  // The stage to ask for next (f_): where its rows begin, its buffers, and which period it opens, whose scales are then to be turned
+  const int v0 = AF == A_E2M1 ? 0 : odd;           // a tile's first stage's step (of e4m3 rows the empty step is no stage)
+  int f_idx = blockIdx.x, f_v = v0, f_ab = 0, f_wb = 0, f_bias = 0, f_period = -1, f_m0, f_n0;
+  const uint8_t *f_a, *f_w, *f_sa, *f_sw;
+  auto fetch_tile = [&]() {
+    tile_at(f_idx, f_m0, f_n0);
+    f_v = v0;
+    f_a = uniform(p.a + ((long)f_m0 * a_ld + (long)(v0 - odd) * (AF == A_E2M1 ? 64 : 128)));
+    f_w = uniform(p.w + ((long)f_n0 * w_ld - odd * 64));
+    f_sa = uniform(p.a_scale + ((long)f_m0 * s_ld - odd * 4));
+    f_sw = uniform(p.w_scale + ((long)f_n0 * s_ld - odd * 4));
+  };
+  fetch_tile();
+  auto fetch = [&]() {
+    f_period = -1;
+    if (f_idx >= nwg) return;
+    const bool first = f_v == v0;
+    issue(f_a, a_off, a_hop, (unsigned)(p.M - 1 - f_m0) * a_ld, f_m0 + BM <= p.M, AF == A_E2M1 && first && odd, std::integral_constant<int, T::A_PER>{},
+          lds0 + (unsigned)(f_ab * T::A_BYTES + w * 1024));
+    f_a += 128;
+    f_ab ^= 1;
+    if (AF == A_E2M1 || (f_v & 1) == 0 || first) {
+      issue(f_w, w_off, w_hop, (unsigned)(p.N - 1 - f_n0) * w_ld, f_n0 + BN <= p.N, first && odd, std::integral_constant<int, T::W_PER>{},
+            lds0 + (unsigned)(T::W_OFF + f_wb * T::W_BYTES + w * 1024));
+      f_w += 128;
+      f_wb ^= 1;
+    }
+    if ((f_v & 3) == 0 || first) {
+      f_period = f_v >> 2;
+      issue_scales(f_sa, f_sw, p.M - f_m0, p.N - f_n0, f_period);
+      f_sa += 16;
+      f_sw += 16;
+    }
+    if (first) {
+      if (p.bias && w < BN / 64)
+        dma4((const uint8_t*)p.bias, (unsigned)min(f_n0 + tid, p.N - 1) * 4u, lds0 + (unsigned)(T::BIAS_OFF + f_bias * BN * 4 + w * 256));
+      f_bias ^= 1;
+    }
+    f_v += T::STEPS;
+    if (f_v >= steps) {
+      f_idx += (int)gridDim.x;
+      if (f_idx < nwg) fetch_tile();
+    }
+  };
+
+  int idx = blockIdx.x, m0, n0;
+  tile_at(idx, m0, n0);
+  int ab = 0, wb = 0, sb = 0, bias_buf = 0;        // the buffers of the current stage, of the current tile's bias
+  fetch();
   WAIT_ALL();
-  scales_store(0);
+  turn_scales(0, 0);
   WAIT_ALL();
   BARRIER();
-  for (int st = 0; st < stages; st += 2) {
-    const int period = st >> 1;
-    const bool more = st + 2 < stages;
-    if (st + 1 < stages) issue(st + 1, 1);
-    if (more) scales_load(period + 1);
-    scales_read(period & 1);
-    MX_STEP(0, 0, 0)
-    if (2 * st + 1 < p.nk) MX_STEP(0, 1, 1)
-    if (st + 1 >= stages) break;
-    WAIT_ALL();
-    if (more) scales_store((period + 1) & 1);
-    WAIT_ALL();
-    BARRIER();
-    if (more) issue(st + 2, 0);
-    MX_STEP(1, 0, 2)
-    if (2 * st + 3 < p.nk) MX_STEP(1, 1, 3)
-    if (!more) break;
-    WAIT_ALL();
-    BARRIER();
-  }
-  WAIT_ALL();
-  BARRIER();                                     // the last stage is read: LDS becomes the waves' images
-
-  // Out: 16 rows x 64 columns of a wave at a time through its own 4 KiB (fp32, 16-byte unit u of row r at u ^ r), so that whole
-  // 128-byte stretches of rows leave and the residual is added before the one rounding.
-  char* img = smem + w * T::IMG;
-  constexpr int JG = T::FN < 4 ? T::FN : 4;      // column fragments of an image
-  const int wave_m = m0 + wm * T::FM * 16, wave_n = n0 + wn * T::FN * 16;
+  fetch();
+  i32x8_t wf[2][FN], af[3];
+  uint32_t sa[3], sw[FN];
+  auto first_fragments = [&](int in_period, i32x8_t (&w_)[FN], i32x8_t& a0, i32x8_t& a1, uint32_t (&sw_)[FN], uint32_t& s0, uint32_t& s1) {
 #pragma unroll
-  for (int jb = 0; jb < T::FN; jb += JG) {
-    f32x4_t bias[JG];
+    for (int j = 0; j < FN; ++j) w_[j] = load_w(wb, in_period, 0, j);
+    a0 = load_a(ab, 0, 0);
 #pragma unroll
-    for (int j = 0; j < JG; ++j)
+    for (int j = 0; j < FN; ++j) sw_[j] = load_scale(sb, in_period, FM * WM + wn * FN + j);
+    s0 = load_scale(sb, in_period, wm * FM);
+    a1 = load_a(ab, 0, 1);
+    s1 = load_scale(sb, in_period, wm * FM + 1);
+  };
+  bool stored = false;                             // the previous tile's STORES stores may still be on their way, issued after the loads
+  while (true) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int n = wave_n + (jb + j) * 16 + g * 4 + e;
-        bias[j][e] = p.bias ? p.bias[min(n, p.N - 1)] : 0.0f;
-      }
+    for (int i = 0; i < FM; ++i)
 #pragma unroll
-    for (int i = 0; i < T::FM; ++i) {
+      for (int j = 0; j < FN; ++j) acc[i][j] = f32x4_t{0, 0, 0, 0};
+    int v = v0;
+    bool last;
+    first_fragments(v0 & 3, wf[0], af[0], af[1], sw, sa[0], sa[1]);   // (not held over the results' way out)
+#pragma clang loop unroll(disable)
+    do {
+      auto products = [&](auto t_) {
+        constexpr int t = decltype(t_)::value, step = t / FM, i = t % FM;
+        __builtin_amdgcn_sched_barrier(0);
+        i32x8_t a = af[t % 3];
+        const int s = (int)sa[t % 3];
+        if constexpr (AF == A_E4M3_BANDS) {
+          const i32x8_t high = high_band(a);
+          a ^= high;
 #pragma unroll
-      for (int j = 0; j < JG; ++j) {
-        f32x4_t v = acc[i][jb + j] + bias[j];
-        if (p.act >= 0) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = activate(v[e], p.act);
+          for (int j = 0; j < FN; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[step][j], high, acc[i][j], 4, 0, step, (int)sw[j], step, s);
         }
-        *(f32x4_t*)(img + r16 * 256 + (((j * 4 + g) ^ r16) << 4)) = v;
-      }
-      asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
-      const int nb = wave_n + jb * 16, mb = wave_m + i * 16;
-      constexpr int COLS = JG * 16;
-      if (nb + COLS <= p.N) {
-        if (p.out_dtype != MX_DT_F32) {
-          constexpr int LPR = COLS / 8;          // lanes a row
 #pragma unroll
-          for (int s = 0; s < 16 * LPR / 64; ++s) {
-            const int row = s * (64 / LPR) + lane / LPR, u = (lane % LPR) * 2;
-            const f32x4_t a = *(const f32x4_t*)(img + row * 256 + ((u ^ row) << 4)), b = *(const f32x4_t*)(img + row * 256 + (((u + 1) ^ row) << 4));
-            const float v[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-            if (mb + row < p.M) store8_16bit(p, (size_t)(mb + row) * p.N + nb + u * 4, v);
-          }
+        for (int j = 0; j < FN; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[step][j], a, acc[i][j], 4, AF != A_E2M1 ? 0 : 4, step, (int)sw[j], step, s);
+        __builtin_amdgcn_sched_barrier(0);
+      };
+      for_each_int<0, N - 2>([&](auto t_) {
+        constexpr int t = decltype(t_)::value, step = t / FM, i = t % FM;
+        af[(t + 2) % 3] = load_a(ab, (t + 2) / FM, (t + 2) % FM);
+        sa[(t + 2) % 3] = load_scale(sb, v & 3, wm * FM + (t + 2) % FM);
+        if constexpr (step + 1 < T::STEPS) {
+#pragma unroll
+          for (int j = 0; j < FN; ++j)
+            if (FM - FN + j == i || (FM < FN && i == 0)) wf[1][j] = load_w(wb, 0, 1, j);
+        }
+        products(t_);
+      });
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) asm volatile("" : "+v"(acc[i][j]));       // the products stay in front of the wait (no instruction)
+      // All of the stage is in registers.  What was asked for a stage ago is the next stage; younger than it are only a finished tile's
+      // results, which need not have left.
+      if (stored) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "i"(T::STORES) : "memory");
+      else WAIT_ALL();
+      stored = false;
+      last = v + T::STEPS >= steps;
+      const int next_v = last ? v0 : v + T::STEPS;
+      if (f_period >= 0) turn_scales(f_period, sb ^ 1);
+      WAIT_LDS();
+      BARRIER();
+      ab ^= 1;
+      if (AF == A_E2M1 || (next_v & 1) == 0 || last) wb ^= 1;
+      if ((next_v & 3) == 0 || last) sb ^= 1;
+      i32x8_t w_next[FN], a0, a1;
+      uint32_t sw_next[FN], s0, s1;
+      first_fragments(next_v & 3, w_next, a0, a1, sw_next, s0, s1);
+      products(std::integral_constant<int, N - 2>{});
+#pragma unroll
+      for (int j = 0; j < FN; ++j) asm volatile("" : "+v"(acc[FM - 2][j]));    // (these stay in front of the asking)
+      fetch();
+      products(std::integral_constant<int, N - 1>{});
+#pragma unroll
+      for (int j = 0; j < FN; ++j) { wf[0][j] = w_next[j]; sw[j] = sw_next[j]; }
+      af[0] = a0; af[1] = a1; sa[0] = s0; sa[1] = s1;
+      v += T::STEPS;
+    } while (!last);
+
+    // Out, straight from the registers: of two neighbouring fragments a lane gets eight neighbouring columns of a row (16 bits), of one
+    // four (fp32); 16 rows x 64 bytes a store
+    int out_lane = lane;
+    asm volatile("" : "+v"(out_lane));             // what follows from it is worked out here, not held in registers over the K loop
+    const int row = m0 + wm * FM * 16 + (out_lane & 15), go = out_lane >> 4;
+    const int col = n0 + wn * FN * 16;
+    const bool whole = m0 + BM <= p.M && n0 + BN <= p.N;
+    f32x4_t bs[FN];
+#pragma unroll
+    for (int j = 0; j < FN; ++j) bs[j] = p.bias ? *(const f32x4_t*)(smem + T::BIAS_OFF + bias_buf * BN * 4 + (wn * FN * 16 + j * 16 + go * 4) * 4) : f32x4_t{0, 0, 0, 0};
+    if (whole && p.out_dtype != MX_DT_F32) {
+      const int c8 = col + 16 * (go & 1) + 8 * (go >> 1);
+      constexpr int HALF = FM / 2;                 // the residual of half the fragments at a time, asked for before any of them is stored
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        u32x4_t r[HALF][FN / 2];
+        if (p.resid) {
+#pragma unroll
+          for (int i = 0; i < HALF; ++i)
+#pragma unroll
+            for (int j = 0; j < FN / 2; ++j)
+              r[i][j] = ((const Pack16*)((const uint16_t*)p.resid + (size_t)(row + (h * HALF + i) * 16) * p.N + c8 + j * 32))->v;
         } else {
-          constexpr int LPR = COLS / 4;
 #pragma unroll
-          for (int s = 0; s < 16 * LPR / 64; ++s) {
-            const int row = s * (64 / LPR) + lane / LPR, u = lane % LPR;
-            f32x4_t v = *(const f32x4_t*)(img + row * 256 + ((u ^ row) << 4));
-            if (mb + row < p.M) {
-              const size_t at = (size_t)(mb + row) * p.N + nb + u * 4;
-              if (p.resid) v += __builtin_bit_cast(f32x4_t, ((const Pack32*)((const float*)p.resid + at))->v);
+          for (int i = 0; i < HALF; ++i)
+#pragma unroll
+            for (int j = 0; j < FN / 2; ++j) r[i][j] = u32x4_t{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int i = 0; i < HALF; ++i) {
+          f32x4_t u[FN];
+#pragma unroll
+          for (int j = 0; j < FN; ++j) u[j] = acc[h * HALF + i][j] + bs[j];
+          activate(u, p.act);
+#pragma unroll
+          for (int j = 0; j < FN / 2; ++j) {
+            pair_columns(u[2 * j], u[2 * j + 1]);
+            Pack16 o;
+            o.v = to_16bit(u[2 * j], u[2 * j + 1], r[i][j], p.resid != nullptr, p.out_dtype);
+            uint16_t* to = (uint16_t*)p.out + (size_t)(row + (h * HALF + i) * 16) * p.N + c8 + j * 32;
+            if (p.streamed) __builtin_nontemporal_store((stream16_t)o.v, (stream16_t*)to);
+            else *(Pack16*)to = o;
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      stored = true;
+    } else {
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+        f32x4_t u[FN];
+#pragma unroll
+        for (int j = 0; j < FN; ++j) u[j] = acc[i][j] + bs[j];
+        activate(u, p.act);
+        const int m = row + i * 16;
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+          const int n = col + j * 16 + go * 4;
+          if (m < p.M && n < p.N) {
+            const size_t at = (size_t)m * p.N + n;
+            if (p.out_dtype == MX_DT_F32 && n + 4 <= p.N) {
+              if (p.resid) u[j] += __builtin_bit_cast(f32x4_t, ((const Pack32*)((const float*)p.resid + at))->v);
               Pack32 o;
-              o.v = __builtin_bit_cast(u32x4_t, v);
+              o.v = __builtin_bit_cast(u32x4_t, u[j]);
               *(Pack32*)((float*)p.out + at) = o;
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (n + e < p.N) store_elem(p.out, at + e, p.out_dtype, p.resid ? u[j][e] + load_elem(p.resid, at + e, p.out_dtype) : u[j][e]);
             }
           }
         }
-      } else {                                   // columns that end inside: a lane a column
-        const int n = nb + lane;
-        for (int row = 0; row < 16; ++row) {
-          const float v = *(const float*)(img + row * 256 + (((lane >> 2) ^ row) << 4) + (lane & 3) * 4);
-          if (lane < COLS && n < p.N && mb + row < p.M) {
-            const size_t at = (size_t)(mb + row) * p.N + n;
-            store_elem(p.out, at, p.out_dtype, p.resid ? v + load_elem(p.resid, at, p.out_dtype) : v);
-          }
-        }
+        __builtin_amdgcn_sched_barrier(0);
       }
-      asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory");
     }
+    bias_buf ^= 1;
+    idx += (int)gridDim.x;
+    if (idx >= nwg) break;
+    tile_at(idx, m0, n0);
   }
 }
 
@@ -346,24 +484,43 @@ template <int AF, int BM, int BN, int WM, int WN>
 hipError_t launch(const MxGemmParams& p, hipStream_t stream) {
   using T = Tile<AF, BM, BN, WM, WN>;
   static DeviceKernelSetup setup;
-  if (hipError_t e = setup.ensure((const void*)mx_gemm_kernel<AF, BM, BN, WM, WN>, T::LDS, nullptr); e != hipSuccess) return e;
+  int n_cu = 0;
+  if (hipError_t e = setup.ensure((const void*)mx_gemm_kernel<AF, BM, BN, WM, WN>, T::LDS, &n_cu); e != hipSuccess) return e;
   const long tiles = (long)((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN);
-  if (tiles > 0x7fffffff) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((mx_gemm_kernel<AF, BM, BN, WM, WN>), dim3((unsigned)tiles), dim3(T::THREADS), T::LDS, stream, p);
+  if (tiles > 0x3fffffff) return hipErrorInvalidValue;
+  const long resident = (long)n_cu * (163840 / T::LDS);             // workgroups that the CUs hold
+  hipLaunchKernelGGL((mx_gemm_kernel<AF, BM, BN, WM, WN>), dim3((unsigned)(tiles < resident ? tiles : resident)), dim3(T::THREADS), T::LDS, stream, p);
   return hipGetLastError();
 }
 
 template <int AF>
-hipError_t choose(const MxGemmParams& p, hipStream_t stream) {
-  constexpr int BIG_M = AF != A_E2M1 ? 128 : 256;
-  const long big = (long)((p.M + BIG_M - 1) / BIG_M) * ((p.N + 255) / 256);
-  if (big >= 256) return launch<AF, BIG_M, 256, 2, 4>(p, stream);
+hipError_t choose(MxGemmParams p, hipStream_t stream) {
+  // 256 x 256 tiles once they give every CU one (256 CUs; a device with fewer only gets them earlier).  Where a last round of them would
+  // leave three quarters of the CUs idle, its rows go to a second launch in small tiles: 65 792 x 4096 -> 1024 is 4 rounds and 4 tiles.
+  constexpr int CUS = 256;
+  const long tn = (p.N + 255) / 256, tiles = (long)((p.M + 255) / 256) * tn;
+  if (tiles < CUS) return launch<AF, 64, 64, 2, 2>(p, stream);
+  const int rest = (int)(tiles % CUS);
+  const long rows = tiles / CUS * CUS / tn * 256;
+  if (rest == 0 || rest * 4 > CUS || rows == 0 || rows >= p.M) return launch<AF, 256, 256, 2, 4>(p, stream);
+  const int M = p.M;
+  p.M = (int)rows;
+  if (hipError_t e = launch<AF, 256, 256, 2, 4>(p, stream); e != hipSuccess) return e;
+  p.M = M - (int)rows;
+  p.a += (size_t)rows * p.nk * (AF == A_E2M1 ? 64 : 128);
+  p.a_scale += (size_t)rows * p.nk * 4;
+  const size_t skip = (size_t)rows * p.N * (p.out_dtype == MX_DT_F32 ? 4 : 2);
+  p.out = (char*)p.out + skip;
+  if (p.resid) p.resid = (const char*)p.resid + skip;
   return launch<AF, 64, 64, 2, 2>(p, stream);
 }
 
 }  // namespace
 
-hipError_t ce_mx_gemm(const MxGemmParams& p, int a_fmt, hipStream_t stream) {
+hipError_t ce_mx_gemm(MxGemmParams p, int a_fmt, hipStream_t stream) {
+  // Results that do not fit the L2s and are not the residual stream's next rows leave with the streaming cache policy: the operands'
+  // panels stay (65 792 x 1024 -> 4096: 265 -> 253 us; onto a residual it costs 1 %).
+  p.streamed = !p.resid && (size_t)p.M * p.N * 2 > (64u << 20);
   if (a_fmt == MX_E2M1) return choose<A_E2M1>(p, stream);
   return p.out_dtype == MX_DT_F32 ? choose<A_E4M3_BANDS>(p, stream) : choose<A_E4M3>(p, stream);
 }

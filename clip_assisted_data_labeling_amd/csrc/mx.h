@@ -11,7 +11,7 @@
 enum { MX_E2M1 = 0, MX_E4M3 = 1, MX_ROW_E4M3 = 2 };
 enum { MX_DT_BF16 = 0, MX_DT_F16 = 1, MX_DT_F32 = 2 };
 enum { MX_NORM_RMS = 0, MX_NORM_LAYER = 1 };
-#define MX_NORM_MAX_K 16384             // widest row of the norm: 512 threads hold it in registers, 32 values each
+#define MX_NORM_MAX_K 16384             // widest row of the norm: 1024 threads hold it in registers, 16 values each
 
 static inline int mx_kp(int k) { return (k + 127) / 128 * 128; }
 
@@ -34,9 +34,10 @@ struct MxGemmParams {
   const void* resid;                          // [M][N] of the output's type, or NULL; may be `out`
   void* out;                                  // [M][N]
   int act, out_dtype;                         // CE_ACT_* or -1; MX_DT_*
+  bool streamed;                              // set by ce_mx_gemm: 16-bit results leave with the streaming cache policy
 };
 
 hipError_t ce_mx_quant(const void* x, int dtype, long n_rows, int k, long ld_x, int fmt, uint8_t* q, uint8_t* scale, hipStream_t stream);
 hipError_t ce_mx_dequant(const uint8_t* q, const void* scale, int fmt, long n_rows, int k, void* out, int out_dtype, hipStream_t stream);
 hipError_t ce_mx_norm(const MxNormParams& p, int dtype, hipStream_t stream);
-hipError_t ce_mx_gemm(const MxGemmParams& p, int a_fmt, hipStream_t stream);
+hipError_t ce_mx_gemm(MxGemmParams p, int a_fmt, hipStream_t stream);

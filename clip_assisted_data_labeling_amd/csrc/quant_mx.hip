@@ -9,10 +9,14 @@
 // All of these kernels move each byte once and are bound by HBM (quantise: 2 bytes in, 0.53 / 1.03 out per value of a 16-bit row).
 // A thread owns 8 consecutive columns -- 16 bytes of a 16-bit row -- and keeps them from row to row, so nothing is divided in the loop;
 // four neighbouring threads share a block (its maximum: two DPP steps), sixteen share the scale word of 128 columns.
+#include <type_traits>
+
 #include "common.h"
 #include "mx.h"
 
 namespace {
+
+constexpr int QUANT_ROWS = 1, QUANT_BLOCKS = 256 * 256, DEQUANT_ROWS = 4, DEQUANT_BLOCKS = 256 * 8;
 
 typedef __attribute__((ext_vector_type(4))) uint32_t u32x4_t;
 typedef __attribute__((ext_vector_type(2))) uint32_t u32x2_t;
@@ -20,62 +24,67 @@ typedef __attribute__((ext_vector_type(2))) uint32_t u32x2_t;
 struct __attribute__((packed, aligned(2))) Pack16 { u32x4_t v; };
 struct __attribute__((packed, aligned(4))) Pack32 { u32x4_t v[2]; };
 
-template <typename T> struct Elem;
-template <> struct Elem<__bf16> {
-  static __device__ __forceinline__ float to_f32(__bf16 v) { return (float)v; }
-  static __device__ __forceinline__ void load8(const __bf16* p, float (&v)[8]) {
-    const u32x4_t r = ((const Pack16*)p)->v;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(r[i] << 16); v[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u); }
-  }
-  static __device__ __forceinline__ void store8(__bf16* p, const float (&v)[8]) {
-    Pack16 r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r.v[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
-    *(Pack16*)p = r;
-  }
-};
-template <> struct Elem<_Float16> {
-  static __device__ __forceinline__ float to_f32(_Float16 v) { return (float)v; }
-  static __device__ __forceinline__ void load8(const _Float16* p, float (&v)[8]) {
-    const f16x8_t r = __builtin_bit_cast(f16x8_t, ((const Pack16*)p)->v);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = (float)r[i];
-  }
-  static __device__ __forceinline__ void store8(_Float16* p, const float (&v)[8]) {
-    f16x8_t r;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) r[i] = (_Float16)v[i];
-    ((Pack16*)p)->v = __builtin_bit_cast(u32x4_t, r);
-  }
-};
-template <> struct Elem<float> {
-  static __device__ __forceinline__ float to_f32(float v) { return v; }
-  static __device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
-    const Pack32 r = *(const Pack32*)p;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r.v[i >> 2][i & 3]);
-  }
-  static __device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
-    Pack32 r;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) r.v[i >> 2][i & 3] = __float_as_uint(v[i]);
-    *(Pack32*)p = r;
-  }
-};
+// Eight values of a row as they lie in memory: 16 or 32 bytes
+template <typename T> struct Raw { u32x4_t v[sizeof(T) / 2]; };
+template <typename T> using Pack = typename std::conditional<sizeof(T) == 2, Pack16, Pack32>::type;
 
-// the columns c .. c + 7 of a row of k; zeros behind its end
-template <typename T>
-__device__ __forceinline__ void load_cols(const T* row, int c, int k, float (&v)[8]) {
-  if (c + 8 <= k) { Elem<T>::load8(row + c, v); return; }
+// The columns c .. c + 7 of a row of k; zeros behind its end.  WHOLE: k % 8 == 0, no chunk is partly behind it.
+template <typename T, bool WHOLE>
+__device__ __forceinline__ Raw<T> load_raw(const T* row, int c, int k) {
+  Raw<T> r;
+  if (c + 8 <= k) {
+    const Pack<T> p = *(const Pack<T>*)(row + c);
+    __builtin_memcpy(&r, &p, sizeof(r));
+    return r;
+  }
+  r = Raw<T>{};
+  if constexpr (!WHOLE) {
+    T e[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = c + i < k ? Elem<T>::to_f32(row[c + i]) : 0.0f;
+    for (int i = 0; i < 8; ++i) e[i] = c + i < k ? row[c + i] : (T)0.0f;
+    __builtin_memcpy(&r, e, sizeof(r));
+  }
+  return r;
+}
+__device__ __forceinline__ void values_of(const Raw<__bf16>& r, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) { v[2 * i] = __uint_as_float(r.v[0][i] << 16); v[2 * i + 1] = __uint_as_float(r.v[0][i] & 0xffff0000u); }
+}
+__device__ __forceinline__ void values_of(const Raw<_Float16>& r, float (&v)[8]) {
+  const f16x8_t h = __builtin_bit_cast(f16x8_t, r.v[0]);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = (float)h[i];
+}
+__device__ __forceinline__ void values_of(const Raw<float>& r, float (&v)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(r.v[i >> 2][i & 3]);
 }
 template <typename T>
-__device__ __forceinline__ void store_cols(T* row, int c, int k, const float (&v)[8]) {
-  if (c + 8 <= k) { Elem<T>::store8(row + c, v); return; }
+__device__ __forceinline__ Raw<T> raw_of(const float (&v)[8]) {
+  Raw<T> r;
+  if constexpr (std::is_same<T, __bf16>::value) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) if (c + i < k) row[c + i] = (T)v[i];
+    for (int i = 0; i < 4; ++i) r.v[0][i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+  } else {
+    T e[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = (T)v[i];
+    __builtin_memcpy(&r, e, sizeof(r));
+  }
+  return r;
+}
+template <typename T, bool WHOLE>
+__device__ __forceinline__ void store_raw(T* row, int c, int k, const Raw<T>& r) {
+  if (c + 8 <= k) {
+    Pack<T> p;
+    __builtin_memcpy(&p, &r, sizeof(r));
+    *(Pack<T>*)(row + c) = p;
+  } else if constexpr (!WHOLE) {
+    T e[8];
+    __builtin_memcpy(e, &r, sizeof(r));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) if (c + i < k) row[c + i] = e[i];
+  }
 }
 
 template <int CTRL>
@@ -146,8 +155,8 @@ __device__ __forceinline__ void store_block(const float (&v)[8], int fmt, uint8_
 }
 
 // Threads 0 .. active - 1 own (row, 8 columns) pairs, row by row; active is a multiple of kp / 8, so that a step of the loop moves
-// every thread by `step` = active / (kp / 8) whole rows.
-template <typename T, int FMT>
+// every thread by `step` = active / (kp / 8) whole rows.  Four rows a thread are in flight.
+template <typename T, int FMT, bool WHOLE>
 __global__ __launch_bounds__(256) void mx_quant_kernel(const T* __restrict__ x, long n_rows, int k, int kp, long ld_x, uint8_t* __restrict__ q,
                                                        uint8_t* __restrict__ scale, long active, long step) {
   const long id = (long)blockIdx.x * 256 + threadIdx.x;
@@ -156,42 +165,59 @@ __global__ __launch_bounds__(256) void mx_quant_kernel(const T* __restrict__ x, 
   const long row0 = id / per_row;
   const int c = (int)(id - row0 * per_row) * 8;
   const size_t q_ld = FMT == MX_E2M1 ? kp / 2 : kp, s_ld = kp / 32;
-  for (long row = row0; row < n_rows; row += step) {
+  constexpr int R = QUANT_ROWS;
+  long row = row0;
+  for (; row + (R - 1) * step < n_rows; row += R * step) {
+    Raw<T> r[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) r[i] = load_raw<T, WHOLE>(x + (row + i * step) * ld_x, c, k);
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      float v[8];
+      values_of(r[i], v);
+      store_block(v, FMT, q + (size_t)(row + i * step) * q_ld, scale + (size_t)(row + i * step) * s_ld, c);
+    }
+  }
+  for (; row < n_rows; row += step) {
     float v[8];
-    load_cols<T>(x + row * ld_x, c, k, v);
+    values_of(load_raw<T, WHOLE>(x + row * ld_x, c, k), v);
     store_block(v, FMT, q + (size_t)row * q_ld, scale + (size_t)row * s_ld, c);
   }
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void mx_dequant_kernel(const uint8_t* __restrict__ q, const void* __restrict__ scale, int fmt, long n_rows, int k,
-                                                         int kp, T* __restrict__ out, long active, long step) {
+__device__ __forceinline__ float scale_value(uint32_t x) {
+  return x == 0xffu ? __builtin_nanf("") : x ? __uint_as_float(x << 23) : 0x1p-127f;
+}
+
+// (row, 8 columns) pairs as above; the elements and scales of four rows are in flight
+template <typename T, int FMT, bool WHOLE>
+__global__ __launch_bounds__(256) void mx_dequant_kernel(const uint8_t* __restrict__ q, const void* __restrict__ scale, long n_rows, int k, int kp,
+                                                         T* __restrict__ out, long active, long step) {
   const long id = (long)blockIdx.x * 256 + threadIdx.x;
   if (id >= active) return;
   const int per_row = kp >> 3;
   const long row0 = id / per_row;
   const int c = (int)(id - row0 * per_row) * 8;
-  const size_t q_ld = fmt == MX_E2M1 ? kp / 2 : kp;
-  for (long row = row0; row < n_rows; row += step) {
-    float s;
-    if (fmt == MX_ROW_E4M3) s = ((const float*)scale)[row];
-    else {
-      const uint32_t x = ((const uint8_t*)scale)[(size_t)row * (kp / 32) + c / 32];
-      s = x == 0xffu ? __builtin_nanf("") : x ? __uint_as_float(x << 23) : 0x1p-127f;
-    }
-    float v[8];
+  if (c >= k) return;
+  const size_t q_ld = FMT == MX_E2M1 ? kp / 2 : kp;
+  auto load = [&](long row, u32x2_t& w, float& s) {
     const uint8_t* src = q + (size_t)row * q_ld;
-    if (fmt == MX_E2M1) {
-      const uint32_t w = *(const uint32_t*)(src + c / 2);
+    if constexpr (FMT == MX_E2M1) w = u32x2_t{*(const uint32_t*)(src + c / 2), 0u};
+    else w = *(const u32x2_t*)(src + c);
+    if constexpr (FMT == MX_ROW_E4M3) s = ((const float*)scale)[row];
+    else s = scale_value(((const uint8_t*)scale)[(size_t)row * (kp / 32) + c / 32]);
+  };
+  auto store = [&](long row, u32x2_t w, float s) {
+    float v[8];
+    if constexpr (FMT == MX_E2M1) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         // the 3-bit magnitude as a float: 0.5 is the format's one subnormal, codes 2 .. 7 are (1 + m / 2) 2^(e - 1)
-        const uint32_t code = (w >> (4 * i)) & 15u, mag = code & 7u;
+        const uint32_t code = (w[0] >> (4 * i)) & 15u, mag = code & 7u;
         const float a = mag < 2u ? 0.5f * (float)mag : __uint_as_float((126u << 23) + (mag << 22));
         v[i] = (code & 8u ? -a : a) * s;
       }
     } else {
-      const u32x2_t w = *(const u32x2_t*)(src + c);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         v[4 * i] = __builtin_amdgcn_cvt_f32_fp8((int)w[i], 0) * s;
@@ -200,16 +226,41 @@ __global__ __launch_bounds__(256) void mx_dequant_kernel(const uint8_t* __restri
         v[4 * i + 3] = __builtin_amdgcn_cvt_f32_fp8((int)w[i], 3) * s;
       }
     }
-    if (c < k) store_cols<T>(out + (size_t)row * k, c, k, v);
+    store_raw<T, WHOLE>(out + (size_t)row * k, c, k, raw_of<T>(v));
+  };
+  constexpr int R = DEQUANT_ROWS;
+  long row = row0;
+  for (; row + (R - 1) * step < n_rows; row += R * step) {
+    u32x2_t w[R];
+    float s[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) load(row + i * step, w[i], s[i]);
+#pragma unroll
+    for (int i = 0; i < R; ++i) store(row + i * step, w[i], s[i]);
+  }
+  for (; row < n_rows; row += step) {
+    u32x2_t w;
+    float s;
+    load(row, w, s);
+    store(row, w, s);
   }
 }
 
 // ---- norm --------------------------------------------------------------------------------------------------------------------------
 //   h = x + resid (rounded to the rows' type, as it is stored);  RMS: y = h / sqrt(mean(h^2) + eps) * gamma + beta,
 //   LAYER: the same of h - mean(h);  then y in blocks, or in e4m3 with one scale a row, max|y| / 448
-// The row stays in the registers of NT threads, CH chunks of 8 columns each.  Sums and the factor are held in 64 bits: fp64 runs
-// at the rate of single fp32 operations here and hides behind the row's bytes, squares cannot overflow, and y is rounded to fp32 once,
-// so that codes differ from the formula's only where y lies within 2^-24 of a rounding border.
+// The row stays in the registers of NT threads, CH chunks of 8 columns each, and so does its share of gamma; the next row's loads are
+// under way while a row is worked on.  Sums, the factor and y are formed in 64 bits -- fp64 runs at the rate of unpacked fp32
+// here and hides behind the row's bytes -- and y reaches its few bits through an fp32 value rounded to ODD, so that codes are those
+// of the 64-bit y: no square overflows, and no value next to a rounding border is rounded twice.
+__device__ __forceinline__ float to_odd(double d) {
+  const float f = (float)d;
+  const double left = d - (double)f;
+  uint32_t b = __float_as_uint(f);
+  if (left != 0.0) b = (b - (((left < 0.0) != (f < 0.0)) ? 1u : 0u)) | 1u;      // |f| > |d|: one step back; inexact: odd
+  return __uint_as_float(b);                                                    // (inf and NaN stay not finite)
+}
+
 template <int NT>
 __device__ __forceinline__ double sum_over(double v, double* red) {
 #pragma unroll
@@ -226,42 +277,57 @@ __device__ __forceinline__ double sum_over(double v, double* red) {
   return v;
 }
 template <int NT>
-__device__ __forceinline__ uint32_t max_over(uint32_t v, uint32_t* red) {
+__device__ __forceinline__ double max_over(double v, double* red) {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o));
+  for (int o = 32; o > 0; o >>= 1) v = fmax(v, __shfl_xor(v, o));
   if constexpr (NT > 64) {
     const int w = threadIdx.x >> 6;
     if ((threadIdx.x & 63) == 0) red[w] = v;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < NT / 64; ++i) v = max(v, red[i]);
+    for (int i = 0; i < NT / 64; ++i) v = fmax(v, red[i]);
     __syncthreads();
   }
   return v;
 }
 
 // NT = 64: four rows a workgroup, one wave each, no barrier;  NT > 64: a row a workgroup
-template <typename T, int NT, int CH>
+template <typename T, int NT, int CH, bool WHOLE, bool ROW>
 __global__ __launch_bounds__(NT == 64 ? 256 : NT) void mx_norm_kernel(const MxNormParams p) {
   __shared__ double red[NT / 64];
   const int t = NT == 64 ? (threadIdx.x & 63) : threadIdx.x;
   const long per_step = NT == 64 ? (long)gridDim.x * 4 : (long)gridDim.x;
   long row = NT == 64 ? (long)blockIdx.x * 4 + (threadIdx.x >> 6) : (long)blockIdx.x;
+  if (row >= p.n_rows) return;                                                  // NT = 64: a whole wave; else the workgroup
+  float g[CH][8];
+#pragma unroll
+  for (int i = 0; i < CH; ++i) values_of(load_raw<float, WHOLE>(p.gamma, (i * NT + t) * 8, p.k), g[i]);
+  auto inside = [&](int i, int j) { return (i * NT + t) * 8 + (WHOLE ? 0 : j) < p.k; };
+  Raw<T> rx[CH], rr[CH];
+  auto fetch = [&](long r) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      rx[i] = load_raw<T, WHOLE>((const T*)p.x + r * p.ld_x, (i * NT + t) * 8, p.k);
+      if (p.resid) rr[i] = load_raw<T, WHOLE>((const T*)p.resid + r * p.ld_r, (i * NT + t) * 8, p.k);
+    }
+  };
+  fetch(row);
   for (; row < p.n_rows; row += per_step) {
     float v[CH][8];
 #pragma unroll
-    for (int i = 0; i < CH; ++i) load_cols<T>((const T*)p.x + row * p.ld_x, (i * NT + t) * 8, p.k, v[i]);
-    if (p.resid) {
-#pragma unroll
-      for (int i = 0; i < CH; ++i) {
-        const int c = (i * NT + t) * 8;
+    for (int i = 0; i < CH; ++i) {
+      values_of(rx[i], v[i]);
+      if (p.resid) {
         float r[8];
-        load_cols<T>((const T*)p.resid + row * p.ld_r, c, p.k, r);
+        values_of(rr[i], r);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] = (float)(T)(v[i][j] + r[j]);
-        if (c < p.k) store_cols<T>((T*)p.h + (size_t)row * p.k, c, p.k, v[i]);
+        for (int j = 0; j < 8; ++j) v[i][j] += r[j];
+        const Raw<T> h = raw_of<T>(v[i]);
+        store_raw<T, WHOLE>((T*)p.h + (size_t)row * p.k, (i * NT + t) * 8, p.k, h);
+        values_of(h, v[i]);
       }
     }
+    if (row + per_step < p.n_rows) fetch(row + per_step);
     double mean = 0;
     if (p.norm == MX_NORM_LAYER) {
       double s = 0;
@@ -276,36 +342,43 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void mx_norm_kernel(const MxNo
     for (int i = 0; i < CH; ++i)
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const double d = (i * NT + t) * 8 + j < p.k ? (double)v[i][j] - mean : 0.0;
+        const double d = inside(i, j) ? (double)v[i][j] - mean : 0.0;
         ss = fma(d, d, ss);
       }
     const double factor = 1.0 / sqrt(sum_over<NT>(ss, red) / p.k + (double)p.eps);
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      const int c = (i * NT + t) * 8;
-      float g[8], b[8];
-      load_cols<float>(p.gamma, c, p.k, g);
-      if (p.beta) load_cols<float>(p.beta, c, p.k, b);
+    auto y_of = [&](int i, double (&y)[8]) {
+      float b[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+      if (p.beta) values_of(load_raw<float, WHOLE>(p.beta, (i * NT + t) * 8, p.k), b);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const double y = ((double)v[i][j] - mean) * factor * (double)g[j] + (p.beta ? (double)b[j] : 0.0);
-        v[i][j] = c + j < p.k ? (float)y : 0.0f;
+        float gj = g[i][j];
+        asm("" : "+v"(gj));                                                     // kept as fp32: its conversion is not to leave the loop
+        y[j] = inside(i, j) ? fma(((double)v[i][j] - mean) * factor, (double)gj, (double)b[j]) : 0.0;
       }
-      m = max(m, abs_bits8(v[i]));
-    }
-    if (p.fmt == MX_ROW_E4M3) {
-      m = max_over<NT>(m, (uint32_t*)red);
-      const float amax = __uint_as_float(m);
-      const bool fine = m < 0x7f800000u;
-      const double inv = m && fine ? 448.0 / (double)amax : 0.0;   // a zero row: scale 0.  In 64 bits: 448 / max may pass fp32's range
-      if (t == 0) ((float*)p.scale)[row] = fine ? amax / 448.0f : __builtin_nanf("");
+    };
+    if constexpr (ROW) {
+      double most = 0, bad = 0;                                                 // fmax drops NaN: it is kept in `bad`
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        double y[8];
+        y_of(i, y);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { most = fmax(most, fabs(y[j])); bad = y[j] - y[j] == 0.0 ? bad : 1.0; }
+      }
+      most = max_over<NT>(most, red);
+      bad = max_over<NT>(bad, red);
+      const bool fine = bad == 0.0 && most <= 3.4028234663852886e38;            // what fp32 holds
+      const double inv = fine && most > 0.0 ? 448.0 / most : 0.0;               // a zero row: scale 0
+      if (t == 0) ((float*)p.scale)[row] = fine ? (float)(most / 448.0) : __builtin_nanf("");
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
         const int c = (i * NT + t) * 8;
+        double y[8];
+        y_of(i, y);
+        float f[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] = (float)((double)v[i][j] * inv);
-        u32x2_t w = to_e4m3(v[i], 1.0f);
+        for (int j = 0; j < 8; ++j) f[j] = to_odd(y[j] * inv);
+        u32x2_t w = to_e4m3(f, 1.0f);
         if (!fine) w = u32x2_t{0u, 0u};
         if (c < p.kp) *(u32x2_t*)(p.q + (size_t)row * p.kp + c) = w;
       }
@@ -314,7 +387,12 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void mx_norm_kernel(const MxNo
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
         const int c = (i * NT + t) * 8;
-        if (c < p.kp) store_block(v[i], p.fmt, p.q + (size_t)row * q_ld, (uint8_t*)p.scale + (size_t)row * (p.kp / 32), c);
+        double y[8];
+        y_of(i, y);
+        float f[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = to_odd(y[j]);
+        if (c < p.kp) store_block(f, p.fmt, p.q + (size_t)row * q_ld, (uint8_t*)p.scale + (size_t)row * (p.kp / 32), c);
       }
     }
   }
@@ -329,27 +407,43 @@ Spread spread_rows(long n_rows, int kp, int blocks) {
   if (rows > n_rows) rows = n_rows;
   return Spread{rows * per_row, rows, (int)((rows * per_row + 255) / 256)};
 }
-constexpr int STREAM_BLOCKS = 256 * 16;
 
 template <typename T>
 void launch_quant(const T* x, long n_rows, int k, long ld_x, int fmt, uint8_t* q, uint8_t* scale, hipStream_t stream) {
   const int kp = mx_kp(k);
-  const Spread s = spread_rows(n_rows, kp, STREAM_BLOCKS);
-  if (fmt == MX_E2M1) hipLaunchKernelGGL((mx_quant_kernel<T, MX_E2M1>), dim3(s.blocks), dim3(256), 0, stream, x, n_rows, k, kp, ld_x, q, scale, s.active, s.step);
-  else hipLaunchKernelGGL((mx_quant_kernel<T, MX_E4M3>), dim3(s.blocks), dim3(256), 0, stream, x, n_rows, k, kp, ld_x, q, scale, s.active, s.step);
+  const Spread s = spread_rows(n_rows, kp, QUANT_BLOCKS);
+#define QUANT_LAUNCH(F, W) hipLaunchKernelGGL((mx_quant_kernel<T, F, W>), dim3(s.blocks), dim3(256), 0, stream, x, n_rows, k, kp, ld_x, q, scale, s.active, s.step)
+  if (k % 8 == 0) { if (fmt == MX_E2M1) QUANT_LAUNCH(MX_E2M1, true); else QUANT_LAUNCH(MX_E4M3, true); }
+  else { if (fmt == MX_E2M1) QUANT_LAUNCH(MX_E2M1, false); else QUANT_LAUNCH(MX_E4M3, false); }
+#undef QUANT_LAUNCH
 }
 
 template <typename T>
+void launch_dequant(const uint8_t* q, const void* scale, int fmt, long n_rows, int k, T* out, hipStream_t stream) {
+  const int kp = mx_kp(k);
+  const Spread s = spread_rows(n_rows, kp, DEQUANT_BLOCKS);
+#define DEQUANT_LAUNCH(F) \
+  if (k % 8 == 0) hipLaunchKernelGGL((mx_dequant_kernel<T, F, true>), dim3(s.blocks), dim3(256), 0, stream, q, scale, n_rows, k, kp, out, s.active, s.step); \
+  else hipLaunchKernelGGL((mx_dequant_kernel<T, F, false>), dim3(s.blocks), dim3(256), 0, stream, q, scale, n_rows, k, kp, out, s.active, s.step)
+  if (fmt == MX_E2M1) { DEQUANT_LAUNCH(MX_E2M1); }
+  else if (fmt == MX_E4M3) { DEQUANT_LAUNCH(MX_E4M3); }
+  else { DEQUANT_LAUNCH(MX_ROW_E4M3); }
+#undef DEQUANT_LAUNCH
+}
+
+template <typename T, bool WHOLE>
 hipError_t launch_norm(const MxNormParams& p, hipStream_t stream) {
   const long waves = (p.n_rows + 3) / 4;
   const int g4 = (int)(waves < 256 * 8 ? waves : 256 * 8), g1 = (int)(p.n_rows < 256 * 8 ? p.n_rows : 256 * 8);
-#define NORM_LAUNCH(NT, CH) hipLaunchKernelGGL((mx_norm_kernel<T, NT, CH>), dim3(NT == 64 ? g4 : g1), dim3(NT == 64 ? 256 : NT), 0, stream, p)
-  if (p.kp <= 512) NORM_LAUNCH(64, 1);
-  else if (p.kp <= 1024) NORM_LAUNCH(64, 2);
-  else if (p.kp <= 2048) NORM_LAUNCH(64, 4);
-  else if (p.kp <= 4096) NORM_LAUNCH(256, 2);
-  else if (p.kp <= 8192) NORM_LAUNCH(256, 4);
-  else if (p.kp <= MX_NORM_MAX_K) NORM_LAUNCH(512, 4);
+#define NORM_LAUNCH(NT, CH) \
+  if (p.fmt == MX_ROW_E4M3) hipLaunchKernelGGL((mx_norm_kernel<T, NT, CH, WHOLE, true>), dim3(NT == 64 ? g4 : g1), dim3(NT == 64 ? 256 : NT), 0, stream, p); \
+  else hipLaunchKernelGGL((mx_norm_kernel<T, NT, CH, WHOLE, false>), dim3(NT == 64 ? g4 : g1), dim3(NT == 64 ? 256 : NT), 0, stream, p)
+  if (p.kp <= 512) { NORM_LAUNCH(64, 1); }
+  else if (p.kp <= 1024) { NORM_LAUNCH(64, 2); }
+  else if (p.kp <= 2048) { NORM_LAUNCH(256, 1); }
+  else if (p.kp <= 4096) { NORM_LAUNCH(512, 1); }
+  else if (p.kp <= 8192) { NORM_LAUNCH(1024, 1); }
+  else if (p.kp <= MX_NORM_MAX_K) { NORM_LAUNCH(1024, 2); }
   else return hipErrorInvalidValue;
 #undef NORM_LAUNCH
   return hipGetLastError();
@@ -365,16 +459,16 @@ hipError_t ce_mx_quant(const void* x, int dtype, long n_rows, int k, long ld_x, 
 }
 
 hipError_t ce_mx_dequant(const uint8_t* q, const void* scale, int fmt, long n_rows, int k, void* out, int out_dtype, hipStream_t stream) {
-  const int kp = mx_kp(k);
-  const Spread s = spread_rows(n_rows, kp, STREAM_BLOCKS);
-#define DEQUANT_LAUNCH(T) hipLaunchKernelGGL((mx_dequant_kernel<T>), dim3(s.blocks), dim3(256), 0, stream, q, scale, fmt, n_rows, k, kp, (T*)out, s.active, s.step)
-  if (out_dtype == MX_DT_BF16) DEQUANT_LAUNCH(__bf16);
-  else if (out_dtype == MX_DT_F16) DEQUANT_LAUNCH(_Float16);
-  else DEQUANT_LAUNCH(float);
-#undef DEQUANT_LAUNCH
+  if (out_dtype == MX_DT_BF16) launch_dequant(q, scale, fmt, n_rows, k, (__bf16*)out, stream);
+  else if (out_dtype == MX_DT_F16) launch_dequant(q, scale, fmt, n_rows, k, (_Float16*)out, stream);
+  else launch_dequant(q, scale, fmt, n_rows, k, (float*)out, stream);
   return hipGetLastError();
 }
 
+template <typename T>
+static hipError_t norm_of(const MxNormParams& p, hipStream_t stream) {
+  return p.k % 8 == 0 ? launch_norm<T, true>(p, stream) : launch_norm<T, false>(p, stream);
+}
 hipError_t ce_mx_norm(const MxNormParams& p, int dtype, hipStream_t stream) {
-  return dtype == MX_DT_BF16 ? launch_norm<__bf16>(p, stream) : dtype == MX_DT_F16 ? launch_norm<_Float16>(p, stream) : launch_norm<float>(p, stream);
+  return dtype == MX_DT_BF16 ? norm_of<__bf16>(p, stream) : dtype == MX_DT_F16 ? norm_of<_Float16>(p, stream) : norm_of<float>(p, stream);
 }

@@ -44,94 +44,116 @@ def _row_bytes(cols: int, fmt: str) -> int:
     return _padded(cols) // 2 if fmt == "e2m1" else _padded(cols)
 
 
+# A call on a few rows costs the host more than the GPU, so the checks below read each attribute once and the stream and the
+# allocations take torch's cheaper forms (a raw stream handle instead of a Stream object, 0.1 against 1.8 us; empty_strided).
+def _stream(device: torch.device) -> int:
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _on_device(index: int):
+    """A guard for work on another device than the current one, None where it is the current one."""
+    return None if index == torch.cuda.current_device() else torch.cuda.device(index)
+
+
+def _run(device: torch.device, what: str, fn, *args) -> None:
+    """fn(*args, stream) on `device`."""
+    guard = _on_device(device.index)
+    if guard is None:
+        rc = fn(*args, _stream(device))
+    else:
+        with guard:
+            rc = fn(*args, _stream(device))
+    if rc:
+        _lib.check(rc, what)
+
+
 def _check_values(what: str, x: torch.Tensor, name: str = "x"):
-    """(dtype code, row stride in elements) of a [rows, cols] matrix of values whose columns lie side by side."""
-    if x.device.type != "cuda":
-        raise _lib.ClipencError(f"{what} needs GPU tensors ('cuda[:i]' under PyTorch-ROCm), got {name} on {x.device}: this build has no CPU path")
-    if x.dtype not in _DTYPES:
+    """(dtype code, device, rows, cols, row stride in elements) of a matrix of values whose columns lie side by side."""
+    device = x.device
+    if device.type != "cuda":
+        raise _lib.ClipencError(f"{what} needs GPU tensors ('cuda[:i]' under PyTorch-ROCm), got {name} on {device}: this build has no CPU path")
+    dt = _DTYPES.get(x.dtype)
+    if dt is None:
         raise ValueError(f"{what}: {name} must be bfloat16, float16 or float32, got {x.dtype}")
-    if x.dim() != 2 or x.shape[1] < 1:
-        raise ValueError(f"{what}: expected {name} of shape [rows, cols], got {tuple(x.shape)}")
-    rows, cols = x.shape
-    if cols > 1 and x.stride(1) != 1:
+    shape = x.shape
+    if len(shape) != 2 or shape[1] < 1:
+        raise ValueError(f"{what}: expected {name} of shape [rows, cols], got {tuple(shape)}")
+    rows, cols = shape
+    ld, step = x.stride()
+    if step != 1 and cols > 1:
         raise ValueError(f"{what}: the columns of {name} must lie side by side (stride 1), got strides {x.stride()}")
-    ld = x.stride(0) if rows > 1 else cols
-    if ld < cols:
+    if rows <= 1:
+        ld = cols
+    elif ld < cols:
         raise ValueError(f"{what}: the rows of {name} overlap (strides {x.stride()})")
-    return _DTYPES[x.dtype], ld
+    return dt, device, rows, cols, ld
 
 
-def _check_quantised(what: str, q: MXTensor, formats, name: str) -> None:
-    if q.fmt not in formats:
-        raise ValueError(f"{what}: {name} must be one of {sorted(formats)}, got {q.fmt!r}")
-    rows, cols = q.data.shape[0], q.cols
-    if cols < 1:
-        raise ValueError(f"{what}: {name} has {cols} columns")
-    want = (rows,) if q.fmt == "e4m3_row" else (rows, _padded(cols) // 32)
-    kind = torch.float32 if q.fmt == "e4m3_row" else torch.uint8
-    if q.data.dtype != torch.uint8 or tuple(q.data.shape) != (rows, _row_bytes(cols, q.fmt)) or q.scale.dtype != kind or tuple(q.scale.shape) != want:
-        raise ValueError(f"{what}: {name} of {cols} columns in {q.fmt} needs uint8 data of {_row_bytes(cols, q.fmt)} bytes a row and {kind} scales "
-                         f"{want}, got {q.data.dtype} {tuple(q.data.shape)} and {q.scale.dtype} {tuple(q.scale.shape)}")
-    if not (q.data.is_contiguous() and q.scale.is_contiguous()):
+def _check_quantised(what: str, q: MXTensor, formats, name: str):
+    """(format code, device, rows, cols) of a quantised matrix."""
+    data, scale, fmt, cols = q
+    if fmt not in formats:
+        raise ValueError(f"{what}: {name} must be one of {sorted(formats)}, got {fmt!r}")
+    kp = (cols + 127) // 128 * 128
+    shape, device = data.shape, data.device
+    rows = shape[0] if len(shape) == 2 else -1
+    row_bytes = kp // 2 if fmt == "e2m1" else kp
+    want, kind = ((rows,), torch.float32) if fmt == "e4m3_row" else ((rows, kp // 32), torch.uint8)
+    if cols < 1 or rows < 0 or shape[1] != row_bytes or data.dtype is not torch.uint8 or scale.dtype is not kind or scale.shape != want:
+        raise ValueError(f"{what}: {name} of {cols} columns in {fmt} needs uint8 data of {row_bytes} bytes a row and {kind} scales {want}, "
+                         f"got {data.dtype} {tuple(shape)} and {scale.dtype} {tuple(scale.shape)}")
+    if not (data.is_contiguous() and scale.is_contiguous()):
         raise ValueError(f"{what}: {name} must be contiguous")
-    if q.data.device.type != "cuda":
-        raise _lib.ClipencError(f"{what} needs GPU tensors, got {name} on {q.data.device}: this build has no CPU path")
+    if device.type != "cuda":
+        raise _lib.ClipencError(f"{what} needs GPU tensors, got {name} on {device}: this build has no CPU path")
+    if scale.device != device:
+        raise ValueError(f"{what}: the data of {name} is on {device}, its scales on {scale.device}")
+    return FORMATS[fmt], device, rows, cols
 
 
-def _check_vector(what: str, v: Optional[torch.Tensor], n: int, name: str) -> Optional[int]:
+def _check_vector(what: str, v: Optional[torch.Tensor], n: int, device: torch.device, name: str) -> Optional[int]:
     if v is None:
         return None
-    if v.dtype != torch.float32 or tuple(v.shape) != (n,) or not v.is_contiguous():
+    if v.dtype is not torch.float32 or v.shape != (n,) or not v.is_contiguous():
         raise ValueError(f"{what}: {name} must be a contiguous float32 [{n}], got {v.dtype} {tuple(v.shape)}")
+    if v.device != device:
+        raise ValueError(f"{what}: all tensors must be on {device}, got {name} on {v.device}")
     return v.data_ptr()
 
 
-def _one_device(what: str, device: torch.device, *tensors) -> None:
-    for t in tensors:
-        if t is not None and t.device != device:
-            raise ValueError(f"{what}: all tensors must be on {device}, got one on {t.device}")
+def _matrix(rows: int, cols: int, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    return torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=device)
 
 
-def _new(rows: int, cols: int, fmt: str, device) -> MXTensor:
-    data = torch.empty((rows, _row_bytes(cols, fmt)), dtype=torch.uint8, device=device)
+def _new(rows: int, cols: int, fmt: str, device: torch.device) -> MXTensor:
+    kp = (cols + 127) // 128 * 128
+    data = _matrix(rows, kp // 2 if fmt == "e2m1" else kp, torch.uint8, device)
     if fmt == "e4m3_row":
-        return MXTensor(data, torch.empty((rows,), dtype=torch.float32, device=device), fmt, cols)
-    return MXTensor(data, torch.empty((rows, _padded(cols) // 32), dtype=torch.uint8, device=device), fmt, cols)
+        return MXTensor(data, torch.empty_strided((rows,), (1,), dtype=torch.float32, device=device), fmt, cols)
+    return MXTensor(data, _matrix(rows, kp // 32, torch.uint8, device), fmt, cols)
 
 
-@torch.no_grad()
 def quantize(x: torch.Tensor, fmt: str = "e2m1") -> MXTensor:
     """The rows of x [rows, cols] (bf16 / fp16 / fp32, rows may be strided) in blocks of 32 columns: fmt "e2m1" or "e4m3"."""
-    if fmt not in ("e2m1", "e4m3"):
+    if fmt != "e2m1" and fmt != "e4m3":
         raise ValueError(f"quantize: fmt must be 'e2m1' or 'e4m3', got {fmt!r}")
-    dt, ld = _check_values("quantize", x)
-    rows, cols = x.shape
-    lib = _lib.load()
-    with torch.cuda.device(x.device):
-        q = _new(rows, cols, fmt, x.device)
-        _lib.check(lib.clipenc_op_quant_mx(x.data_ptr(), dt, rows, cols, ld, FORMATS[fmt], q.data.data_ptr(), q.scale.data_ptr(),
-                                           _lib.current_stream_ptr(x.device)), "quantize")
+    dt, device, rows, cols, ld = _check_values("quantize", x)
+    q = _new(rows, cols, fmt, device)
+    _run(device, "quantize", _lib.load().clipenc_op_quant_mx, x.data_ptr(), dt, rows, cols, ld, FORMATS[fmt], q.data.data_ptr(), q.scale.data_ptr())
     return q
 
 
-@torch.no_grad()
 def dequantize(q: MXTensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The values [rows, cols] that q stands for."""
-    if dtype not in _DTYPES:
+    out_dt = _DTYPES.get(dtype)
+    if out_dt is None:
         raise ValueError(f"dequantize: dtype must be bfloat16, float16 or float32, got {dtype}")
-    _check_quantised("dequantize", q, FORMATS, "q")
-    device = q.data.device
-    _one_device("dequantize", device, q.scale)
-    rows, cols = q.shape
-    lib = _lib.load()
-    with torch.cuda.device(device):
-        out = torch.empty((rows, cols), dtype=dtype, device=device)
-        _lib.check(lib.clipenc_op_dequant_mx(q.data.data_ptr(), q.scale.data_ptr(), FORMATS[q.fmt], rows, cols, out.data_ptr(), _DTYPES[dtype],
-                                             _lib.current_stream_ptr(device)), "dequantize")
+    fmt, device, rows, cols = _check_quantised("dequantize", q, FORMATS, "q")
+    out = _matrix(rows, cols, dtype, device)
+    _run(device, "dequantize", _lib.load().clipenc_op_dequant_mx, q.data.data_ptr(), q.scale.data_ptr(), fmt, rows, cols, out.data_ptr(), out_dt)
     return out
 
 
-@torch.no_grad()
 def norm_quantize(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
                   norm: str = "rms", eps: float = 1e-6, fmt: str = "e4m3") -> Tuple[torch.Tensor, MXTensor]:
     """(h, q): h = x + residual (x itself without one), q = its norm ("rms" or "layer") times `weight` plus `bias`, quantised to fmt:
@@ -139,28 +161,24 @@ def norm_quantize(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
     what = "norm_quantize"
     if norm not in NORMS or fmt not in FORMATS:
         raise ValueError(f"{what}: norm must be one of {sorted(NORMS)} and fmt one of {sorted(FORMATS)}, got {norm!r}, {fmt!r}")
-    dt, ld = _check_values(what, x)
-    rows, cols = x.shape
-    ld_r = 0
+    dt, device, rows, cols, ld = _check_values(what, x)
+    r = hp = None
+    ld_r, h = 0, x
     if residual is not None:
-        dt_r, ld_r = _check_values(what, residual, "residual")
-        if residual.shape != x.shape or dt_r != dt:
-            raise ValueError(f"{what}: residual must be {x.dtype} {tuple(x.shape)}, got {residual.dtype} {tuple(residual.shape)}")
+        if residual.shape != x.shape or residual.dtype is not x.dtype or residual.device != device:
+            raise ValueError(f"{what}: residual must be {x.dtype} {tuple(x.shape)} on {device}, got {residual.dtype} {tuple(residual.shape)} on {residual.device}")
+        ld_r = _check_values(what, residual, "residual")[4]
+        h = _matrix(rows, cols, x.dtype, device)
+        r, hp = residual.data_ptr(), h.data_ptr()
     if weight is None:
         raise ValueError(f"{what}: weight is needed")
-    g, b = _check_vector(what, weight, cols, "weight"), _check_vector(what, bias, cols, "bias")
-    _one_device(what, x.device, weight, bias, residual)
-    lib = _lib.load()
-    with torch.cuda.device(x.device):
-        h = x if residual is None else torch.empty((rows, cols), dtype=x.dtype, device=x.device)
-        q = _new(rows, cols, fmt, x.device)
-        _lib.check(lib.clipenc_op_norm_quant_mx(x.data_ptr(), dt, rows, cols, ld, None if residual is None else residual.data_ptr(), ld_r,
-                                                NORMS[norm], g, b, eps, FORMATS[fmt], None if residual is None else h.data_ptr(),
-                                                q.data.data_ptr(), q.scale.data_ptr(), _lib.current_stream_ptr(x.device)), what)
+    g, b = _check_vector(what, weight, cols, device, "weight"), _check_vector(what, bias, cols, device, "bias")
+    q = _new(rows, cols, fmt, device)
+    _run(device, what, _lib.load().clipenc_op_norm_quant_mx, x.data_ptr(), dt, rows, cols, ld, r, ld_r, NORMS[norm], g, b, eps, FORMATS[fmt], hp,
+         q.data.data_ptr(), q.scale.data_ptr())
     return h, q
 
 
-@torch.no_grad()
 def linear(x, w: MXTensor, bias: Optional[torch.Tensor] = None, act: Optional[str] = None, residual: Optional[torch.Tensor] = None,
            out_dtype: Optional[torch.dtype] = None, x_fmt: str = "e4m3") -> torch.Tensor:
     """act(x . w^T + bias) + residual, [rows, out].  x: an MXTensor ("e4m3" or "e2m1") or values [rows, cols], which are quantised to
@@ -171,39 +189,37 @@ def linear(x, w: MXTensor, bias: Optional[torch.Tensor] = None, act: Optional[st
         raise ValueError(f"{what}: act must be None, 'quick_gelu' or 'gelu', got {act!r}")
     if act is not None and residual is not None:
         raise ValueError(f"{what}: activation and residual are exclusive")
-    _check_quantised(what, w, ("e2m1",), "w")
+    _, device, n, w_cols = _check_quantised(what, w, ("e2m1",), "w")
     coded = isinstance(x, MXTensor)
     if coded:
-        _check_quantised(what, x, ("e2m1", "e4m3"), "x")
-        device = x.data.device
+        fmt, x_device, rows, cols = _check_quantised(what, x, ("e2m1", "e4m3"), "x")
     else:
-        if x_fmt not in ("e2m1", "e4m3"):
+        if x_fmt != "e2m1" and x_fmt != "e4m3":
             raise ValueError(f"{what}: x_fmt must be 'e2m1' or 'e4m3', got {x_fmt!r}")
-        dt, ld = _check_values(what, x)
-        device = x.device
-    rows, cols = x.shape
-    n = w.data.shape[0]
-    if cols != w.cols:
-        raise ValueError(f"{what}: x has {cols} columns and w {w.cols}")
-    out_dtype = out_dtype or (torch.bfloat16 if coded else x.dtype)
-    if out_dtype not in _DTYPES:
+        fmt = FORMATS[x_fmt]
+        dt, x_device, rows, cols, ld = _check_values(what, x)
+    if x_device != device:
+        raise ValueError(f"{what}: x is on {x_device} and w on {device}")
+    if cols != w_cols:
+        raise ValueError(f"{what}: x has {cols} columns and w {w_cols}")
+    if out_dtype is None:
+        out_dtype = torch.bfloat16 if coded else x.dtype
+    out_dt = _DTYPES.get(out_dtype)
+    if out_dt is None:
         raise ValueError(f"{what}: out_dtype must be bfloat16, float16 or float32, got {out_dtype}")
-    b = _check_vector(what, bias, n, "bias")
-    if residual is not None and (residual.dtype != out_dtype or tuple(residual.shape) != (rows, n) or not residual.is_contiguous()):
-        raise ValueError(f"{what}: residual must be a contiguous {out_dtype} [{rows}, {n}], got {residual.dtype} {tuple(residual.shape)}")
-    _one_device(what, device, w.data, w.scale, bias, residual, *((x.scale,) if coded else ()))
-    r = None if residual is None else residual.data_ptr()
+    b, r = _check_vector(what, bias, n, device, "bias"), None
+    if residual is not None:
+        if residual.dtype is not out_dtype or residual.shape != (rows, n) or not residual.is_contiguous() or residual.device != device:
+            raise ValueError(f"{what}: residual must be a contiguous {out_dtype} [{rows}, {n}] on {device}, got {residual.dtype} {tuple(residual.shape)} on {residual.device}")
+        r = residual.data_ptr()
     lib = _lib.load()
-    with torch.cuda.device(device):
-        out = torch.empty((rows, n), dtype=out_dtype, device=device)
-        stream = _lib.current_stream_ptr(device)
-        if coded:
-            _lib.check(lib.clipenc_op_gemm_mx(x.data.data_ptr(), x.scale.data_ptr(), FORMATS[x.fmt], w.data.data_ptr(), w.scale.data_ptr(), rows, n,
-                                              cols, b, ACTS[act], r, out.data_ptr(), _DTYPES[out_dtype], stream), what)
-        else:
-            need = lib.clipenc_op_linear_mx_ws_bytes(rows, cols, FORMATS[x_fmt])
-            ws = torch.empty((need,), dtype=torch.uint8, device=device) if need else None
-            _lib.check(lib.clipenc_op_linear_mx(x.data_ptr(), dt, ld, FORMATS[x_fmt], w.data.data_ptr(), w.scale.data_ptr(), rows, n, cols, b,
-                                                ACTS[act], r, out.data_ptr(), _DTYPES[out_dtype], None if ws is None else ws.data_ptr(), need,
-                                                stream), what)
+    out = _matrix(rows, n, out_dtype, device)
+    if coded:
+        _run(device, what, lib.clipenc_op_gemm_mx, x.data.data_ptr(), x.scale.data_ptr(), fmt, w.data.data_ptr(), w.scale.data_ptr(), rows, n, cols, b,
+             ACTS[act], r, out.data_ptr(), out_dt)
+    else:
+        need = lib.clipenc_op_linear_mx_ws_bytes(rows, cols, fmt)
+        ws = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=device) if need else None
+        _run(device, what, lib.clipenc_op_linear_mx, x.data_ptr(), dt, ld, fmt, w.data.data_ptr(), w.scale.data_ptr(), rows, n, cols, b, ACTS[act], r,
+             out.data_ptr(), out_dt, ws.data_ptr() if need else None, need)
     return out

@@ -253,7 +253,7 @@ def test_linear_of_quantised_rows(gpu, m, n, k, fmt):
 
 
 @pytest.mark.parametrize("fmt", ["e2m1", "e4m3"])
-@pytest.mark.parametrize("m,n,k", [(4100, 4090, 200), (4097, 4104, 640), (8300, 2048, 1152), (700, 900, 384), (1500, 1280, 256)])
+@pytest.mark.parametrize("m,n,k", [(4100, 4090, 200), (4097, 4104, 640), (8300, 2048, 1152), (5600, 4090, 300), (5601, 4096, 640), (700, 900, 384), (1500, 1280, 256)])
 def test_linear_of_many_rows(gpu, m, n, k, fmt):
     a, av = _random_coded(m, k, fmt, 1, gpu)
     w, wv = _random_coded(n, k, "e2m1", 2, gpu)
