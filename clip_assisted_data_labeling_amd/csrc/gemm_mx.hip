@@ -480,6 +480,171 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mx_gemm_kernel(const MxGemmPa
   }
 }
 
+// ---- few rows -----------------------------------------------------------------------------------------------------------------------
+// Up to 64 rows: 16 columns n a workgroup, whose waves share K and add their sums up in LDS, in wave order.  Fragments come straight from
+// memory -- each byte of W is read once, and there is nothing to wait for but that one read: a tile walk of the same product pays a
+// memory latency a stage.  SRC: quantised rows (MX_E2M1 / MX_E4M3), or values of type T that the lanes quantise themselves, with the
+// codes of clipenc_op_quant_mx (up to 16 rows: each workgroup does it again).
+struct MxFewParams {
+  MxGemmParams g;
+  const void* x; long ld_x; int k;                // values: [M] rows of k
+};
+
+// A lane's 32 values as they lie in a fragment -> its 4 or 8 words and its block's scale byte.  e2m1: block g, columns 32 g .. 32 g + 31.
+// e4m3: 16 columns of block g / 2 and 16 of block 2 + g / 2, shared with lane ^ 16; the scale of block g comes from a lane that has it.
+__device__ __forceinline__ i32x8_t quantise_fragment(const float (&v)[32], int fmt, uint32_t& scale) {
+  uint32_t m[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 32; ++i) m[i >> 4] = max(m[i >> 4], __float_as_uint(v[i]) & 0x7fffffffu);
+  i32x8_t q = {0, 0, 0, 0, 0, 0, 0, 0};
+  if (fmt == MX_E2M1) {
+    float inv;
+    scale = mx_block_scale(max(m[0], m[1]), 2, inv);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w = mx_to_e2m1(v + 8 * i, inv);
+      q[i] = scale == 0xffu ? 0 : (int)w;
+    }
+  } else {
+    uint32_t x[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float inv;
+      x[h] = mx_block_scale(max(m[h], (uint32_t)__shfl_xor((int)m[h], 16)), 8, inv);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const mx_u32x2_t w = mx_to_e4m3(v + 16 * h + 8 * i, inv);
+        q[4 * h + 2 * i] = x[h] == 0xffu ? 0 : (int)w[0];
+        q[4 * h + 2 * i + 1] = x[h] == 0xffu ? 0 : (int)w[1];
+      }
+    }
+    const int lane = threadIdx.x & 63, g = lane >> 4;
+    const uint32_t both = (uint32_t)__shfl((int)(x[0] | x[1] << 8), (lane & 15) + (g == 1 ? 32 : g == 2 ? 0 : 16 * g));
+    scale = g < 2 ? both & 0xffu : both >> 8;
+  }
+  return q;
+}
+// the columns c .. c + 15 of a row of k as floats, zeros behind its end
+template <typename T>
+__device__ __forceinline__ void load16(const T* row, int c, int k, float* v) {
+  constexpr int PACKS = sizeof(T) / 2 * 2, PER = 16 / PACKS;                       // 16-byte packs, values in each
+  if (c + 16 <= k) {
+#pragma unroll
+    for (int i = 0; i < PACKS; ++i) {
+      u32x4_t r;
+      if constexpr (sizeof(T) == 2) r = ((const Pack16*)(row + c + i * PER))->v;
+      else r = ((const Pack32*)(row + c + i * PER))->v;
+      if constexpr (std::is_same<T, __bf16>::value) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { v[8 * i + 2 * e] = __uint_as_float(r[e] << 16); v[8 * i + 2 * e + 1] = __uint_as_float(r[e] & 0xffff0000u); }
+      } else if constexpr (std::is_same<T, _Float16>::value) {
+        const f16x8_t h = __builtin_bit_cast(f16x8_t, r);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[8 * i + e] = (float)h[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[4 * i + e] = __uint_as_float(r[e]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = c + i < k ? (float)row[c + i] : 0.0f;
+  }
+}
+
+constexpr int FEW_WAVES = 8;
+
+// T = void: the rows are quantised;  AF: A_*;  MF: 16-row fragments
+template <typename T, int AF, int MF>
+__global__ __launch_bounds__(FEW_WAVES * 64) void mx_few_kernel(const MxFewParams fp) {
+  const MxGemmParams& p = fp.g;
+  constexpr bool VALUES = !std::is_same<T, void>::value;
+  constexpr int FMT = AF == A_E2M1 ? MX_E2M1 : MX_E4M3;
+  __shared__ __attribute__((aligned(16))) float sums[FEW_WAVES][MF][256];
+  const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6), waves = blockDim.x >> 6;
+  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * (MF * 16);
+  const size_t w_row = (size_t)min(n0 + r16, p.N - 1) * p.nk;                      // in K steps
+  f32x4_t acc[MF];
+#pragma unroll
+  for (int i = 0; i < MF; ++i) acc[i] = f32x4_t{0, 0, 0, 0};
+  constexpr int U = VALUES ? 2 : MF == 1 ? 4 : 2;                                  // K steps in flight
+  for (int ks0 = w; ks0 < p.nk; ks0 += U * waves) {
+    i32x8_t wf[U], af[U][MF];
+    uint32_t sw[U], sa[U][MF];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int ks = min(ks0 + u * waves, p.nk - 1);                               // (behind the end: that step again, not multiplied)
+      const i32x4_t v = *(const i32x4_t*)(p.w + (w_row + ks) * 64 + g * 16);
+      wf[u] = __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1);
+      sw[u] = p.w_scale[(w_row + ks) * 4 + g];
+#pragma unroll
+      for (int i = 0; i < MF; ++i) {
+        const size_t row = (size_t)min(m0 + i * 16 + r16, p.M - 1);
+        if constexpr (VALUES) {
+          const T* x = (const T*)fp.x + row * fp.ld_x;
+          float f[32];
+          if (FMT == MX_E2M1) {
+            load16(x, ks * 128 + g * 32, fp.k, f);
+            load16(x, ks * 128 + g * 32 + 16, fp.k, f + 16);
+          } else {
+            load16(x, ks * 128 + g * 16, fp.k, f);
+            load16(x, ks * 128 + 64 + g * 16, fp.k, f + 16);
+          }
+          af[u][i] = quantise_fragment(f, FMT, sa[u][i]);
+        } else {
+          sa[u][i] = p.a_scale[(row * p.nk + ks) * 4 + g];
+          if constexpr (AF == A_E2M1) {
+            const i32x4_t q = *(const i32x4_t*)(p.a + (row * p.nk + ks) * 64 + g * 16);
+            af[u][i] = __builtin_shufflevector(q, q, 0, 1, 2, 3, -1, -1, -1, -1);
+          } else {
+            const uint8_t* q = p.a + (row * p.nk + ks) * 128 + g * 16;
+            const i32x4_t lo = *(const i32x4_t*)q, hi = *(const i32x4_t*)(q + 64);
+            af[u][i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (ks0 + u * waves >= p.nk) break;                                          // (the same for the whole wave)
+#pragma unroll
+      for (int i = 0; i < MF; ++i) {
+        i32x8_t a = af[u][i];
+        if constexpr (AF == A_E4M3_BANDS) {
+          const i32x8_t high = high_band(a);
+          a ^= high;
+          acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[u], high, acc[i], 4, 0, 0, (int)sw[u], 0, (int)sa[u][i]);
+        }
+        acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[u], a, acc[i], 4, AF != A_E2M1 ? 0 : 4, 0, (int)sw[u], 0, (int)sa[u][i]);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < MF; ++i) *(f32x4_t*)&sums[w][i][r16 * 16 + g * 4] = acc[i];   // row r16, columns 4 g .. 4 g + 3
+  __syncthreads();
+  for (int t = tid; t < MF * 256; t += blockDim.x) {
+    const int m = m0 + t / 16, n = n0 + (t & 15);
+    float v = 0.0f;
+    for (int i = 0; i < waves; ++i) v += sums[i][t / 256][t & 255];
+    if (m < p.M && n < p.N) {
+      if (p.bias) v += p.bias[n];
+      f32x4_t one[1] = {f32x4_t{v, v, v, v}};
+      activate(one, p.act);
+      const size_t at = (size_t)m * p.N + n;
+      store_elem(p.out, at, p.out_dtype, p.resid ? one[0][0] + load_elem(p.resid, at, p.out_dtype) : one[0][0]);
+    }
+  }
+}
+
+template <typename T, int AF, int MF>
+hipError_t launch_few(const MxFewParams& p, hipStream_t stream) {
+  const int waves = p.g.nk < FEW_WAVES ? p.g.nk : FEW_WAVES;
+  hipLaunchKernelGGL((mx_few_kernel<T, AF, MF>), dim3((unsigned)((p.g.N + 15) / 16), (unsigned)((p.g.M + MF * 16 - 1) / (MF * 16))), dim3((unsigned)waves * 64), 0,
+                     stream, p);
+  return hipGetLastError();
+}
+
 template <int AF, int BM, int BN, int WM, int WN>
 hipError_t launch(const MxGemmParams& p, hipStream_t stream) {
   using T = Tile<AF, BM, BN, WM, WN>;
@@ -495,6 +660,11 @@ hipError_t launch(const MxGemmParams& p, hipStream_t stream) {
 
 template <int AF>
 hipError_t choose(MxGemmParams p, hipStream_t stream) {
+  if (p.M <= MX_FEW_ROWS) {
+    MxFewParams f{};
+    f.g = p;
+    return p.M <= 16 ? launch_few<void, AF, 1>(f, stream) : p.M <= 32 ? launch_few<void, AF, 2>(f, stream) : launch_few<void, AF, 4>(f, stream);
+  }
   // 256 x 256 tiles once they give every CU one (256 CUs; a device with fewer only gets them earlier).  Where a last round of them would
   // leave three quarters of the CUs idle, its rows go to a second launch in small tiles: 65 792 x 4096 -> 1024 is 4 rounds and 4 tiles.
   constexpr int CUS = 256;
@@ -523,4 +693,16 @@ hipError_t ce_mx_gemm(MxGemmParams p, int a_fmt, hipStream_t stream) {
   p.streamed = !p.resid && (size_t)p.M * p.N * 2 > (64u << 20);
   if (a_fmt == MX_E2M1) return choose<A_E2M1>(p, stream);
   return p.out_dtype == MX_DT_F32 ? choose<A_E4M3_BANDS>(p, stream) : choose<A_E4M3>(p, stream);
+}
+
+template <typename T>
+static hipError_t few_values(const MxFewParams& f, int fmt, hipStream_t stream) {
+  if (fmt == MX_E2M1) return launch_few<T, A_E2M1, 1>(f, stream);
+  return f.g.out_dtype == MX_DT_F32 ? launch_few<T, A_E4M3_BANDS, 1>(f, stream) : launch_few<T, A_E4M3, 1>(f, stream);
+}
+hipError_t ce_mx_gemm_values(const MxGemmParams& p, const void* x, int dtype, long ld_x, int k, int fmt, hipStream_t stream) {
+  if (p.M > MX_VALUE_ROWS) return hipErrorInvalidValue;
+  MxFewParams f{};
+  f.g = p; f.x = x; f.ld_x = ld_x; f.k = k;
+  return dtype == MX_DT_BF16 ? few_values<__bf16>(f, fmt, stream) : dtype == MX_DT_F16 ? few_values<_Float16>(f, fmt, stream) : few_values<float>(f, fmt, stream);
 }

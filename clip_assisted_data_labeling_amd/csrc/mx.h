@@ -13,6 +13,9 @@ enum { MX_DT_BF16 = 0, MX_DT_F16 = 1, MX_DT_F32 = 2 };
 enum { MX_NORM_RMS = 0, MX_NORM_LAYER = 1 };
 #define MX_NORM_MAX_K 16384             // widest row of the norm: 1024 threads hold it in registers, 16 values each
 
+#define MX_FEW_ROWS 64                  // products of so few rows read their fragments straight from memory
+#define MX_VALUE_ROWS 16                // products of so few rows take values and quantise them themselves
+
 static inline int mx_kp(int k) { return (k + 127) / 128 * 128; }
 
 struct MxNormParams {
@@ -37,7 +40,43 @@ struct MxGemmParams {
   bool streamed;                              // set by ce_mx_gemm: 16-bit results leave with the streaming cache policy
 };
 
+#ifdef __HIPCC__
+typedef __attribute__((ext_vector_type(2))) uint32_t mx_u32x2_t;
+// eight values times `inv` (a power of two, or the row's 448 / max) to e4m3 / e2m1; v_cvt_pk_fp8_f32 does not saturate, the e2m1 one does
+__device__ __forceinline__ mx_u32x2_t mx_to_e4m3(const float* v, float inv) {
+  float q[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) q[i] = __builtin_amdgcn_fmed3f(v[i] * inv, -448.0f, 448.0f);
+  int a = 0, b = 0;
+  a = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], a, false);
+  a = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], a, true);
+  b = __builtin_amdgcn_cvt_pk_fp8_f32(q[4], q[5], b, false);
+  b = __builtin_amdgcn_cvt_pk_fp8_f32(q[6], q[7], b, true);
+  return mx_u32x2_t{(uint32_t)a, (uint32_t)b};
+}
+__device__ __forceinline__ uint32_t mx_to_e2m1(const float* v, float inv) {
+  uint32_t w = 0;
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[0] * inv, v[1] * inv, 1.0f, 0);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[2] * inv, v[3] * inv, 1.0f, 1);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[4] * inv, v[5] * inv, 1.0f, 2);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[6] * inv, v[7] * inv, 1.0f, 3);
+  return w;
+}
+
+// The scale byte and 1 / 2^X of a block whose largest magnitude has the bits `m`.
+__device__ __forceinline__ uint32_t mx_block_scale(uint32_t m, int emax, float& inv) {
+  if (m >= 0x7f800000u) { inv = 0.0f; return 0xffu; }
+  int e = (int)(m >> 23) - 127;
+  if (m < 0x00800000u) e = m ? (31 - __clz((int)m)) - 149 : -127;   // subnormal maxima: fp32 inputs only
+  const int x = max(e - emax, -127);                                 // <= 125
+  inv = __uint_as_float((uint32_t)(127 - x) << 23);                  // 2^-X, X in [-127, 125]: a normal float
+  return (uint32_t)(x + 127);
+}
+#endif
+
 hipError_t ce_mx_quant(const void* x, int dtype, long n_rows, int k, long ld_x, int fmt, uint8_t* q, uint8_t* scale, hipStream_t stream);
 hipError_t ce_mx_dequant(const uint8_t* q, const void* scale, int fmt, long n_rows, int k, void* out, int out_dtype, hipStream_t stream);
 hipError_t ce_mx_norm(const MxNormParams& p, int dtype, hipStream_t stream);
 hipError_t ce_mx_gemm(MxGemmParams p, int a_fmt, hipStream_t stream);
+// p.M <= MX_VALUE_ROWS: the rows of p.a are quantised from x inside
+hipError_t ce_mx_gemm_values(const MxGemmParams& p, const void* x, int dtype, long ld_x, int k, int fmt, hipStream_t stream);

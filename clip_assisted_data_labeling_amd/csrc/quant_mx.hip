@@ -19,7 +19,7 @@ namespace {
 constexpr int QUANT_ROWS = 1, QUANT_BLOCKS = 256 * 256, DEQUANT_ROWS = 4, DEQUANT_BLOCKS = 256 * 8;
 
 typedef __attribute__((ext_vector_type(4))) uint32_t u32x4_t;
-typedef __attribute__((ext_vector_type(2))) uint32_t u32x2_t;
+typedef mx_u32x2_t u32x2_t;
 // rows start at any element: the vector accesses promise no more than the element's own alignment (gfx950 takes them all)
 struct __attribute__((packed, aligned(2))) Pack16 { u32x4_t v; };
 struct __attribute__((packed, aligned(4))) Pack32 { u32x4_t v[2]; };
@@ -101,37 +101,6 @@ __device__ __forceinline__ uint32_t abs_bits8(const float (&v)[8]) {
   return m;
 }
 
-// eight values times `inv` (a power of two, or the row's 448 / max) to e4m3 / e2m1; v_cvt_pk_fp8_f32 does not saturate, the e2m1 one does
-__device__ __forceinline__ u32x2_t to_e4m3(const float (&v)[8], float inv) {
-  float q[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) q[i] = __builtin_amdgcn_fmed3f(v[i] * inv, -448.0f, 448.0f);
-  int a = 0, b = 0;
-  a = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], a, false);
-  a = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], a, true);
-  b = __builtin_amdgcn_cvt_pk_fp8_f32(q[4], q[5], b, false);
-  b = __builtin_amdgcn_cvt_pk_fp8_f32(q[6], q[7], b, true);
-  return u32x2_t{(uint32_t)a, (uint32_t)b};
-}
-__device__ __forceinline__ uint32_t to_e2m1(const float (&v)[8], float inv) {
-  uint32_t w = 0;
-  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[0] * inv, v[1] * inv, 1.0f, 0);
-  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[2] * inv, v[3] * inv, 1.0f, 1);
-  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[4] * inv, v[5] * inv, 1.0f, 2);
-  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, v[6] * inv, v[7] * inv, 1.0f, 3);
-  return w;
-}
-
-// The scale byte and 1 / 2^X of a block whose largest magnitude has the bits `m`.
-__device__ __forceinline__ uint32_t block_scale(uint32_t m, int emax, float& inv) {
-  if (m >= 0x7f800000u) { inv = 0.0f; return 0xffu; }
-  int e = (int)(m >> 23) - 127;
-  if (m < 0x00800000u) e = m ? (31 - __clz((int)m)) - 149 : -127;   // subnormal maxima: fp32 inputs only
-  const int x = max(e - emax, -127);                                 // <= 125
-  inv = __uint_as_float((uint32_t)(127 - x) << 23);                  // 2^-X, X in [-127, 125]: a normal float
-  return (uint32_t)(x + 127);
-}
-
 // Quantises the thread's 8 columns; the 16 threads of 128 columns take part together.  Non-finite blocks: inf * 0 would be NaN, so
 // their elements are cleared.
 __device__ __forceinline__ void store_block(const float (&v)[8], int fmt, uint8_t* q_row, uint8_t* s_row, int c) {
@@ -139,15 +108,15 @@ __device__ __forceinline__ void store_block(const float (&v)[8], int fmt, uint8_
   m = max(m, dpp<DPP_XOR1>(m));
   m = max(m, dpp<DPP_XOR2>(m));
   float inv;
-  const uint32_t x = block_scale(m, fmt == MX_E2M1 ? 2 : 8, inv);
+  const uint32_t x = mx_block_scale(m, fmt == MX_E2M1 ? 2 : 8, inv);
   uint32_t word = x << (8 * ((threadIdx.x >> 2) & 3));
   word |= dpp<DPP_HALF_MIRROR>(word);
   word |= dpp<DPP_MIRROR>(word);
   if (fmt == MX_E2M1) {
-    const uint32_t w = to_e2m1(v, inv);
+    const uint32_t w = mx_to_e2m1(v, inv);
     *(uint32_t*)(q_row + c / 2) = x == 0xffu ? 0u : w;
   } else {
-    u32x2_t w = to_e4m3(v, inv);
+    u32x2_t w = mx_to_e4m3(v, inv);
     if (x == 0xffu) w = u32x2_t{0u, 0u};
     *(u32x2_t*)(q_row + c) = w;
   }
@@ -378,7 +347,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void mx_norm_kernel(const MxNo
         float f[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) f[j] = to_odd(y[j] * inv);
-        u32x2_t w = to_e4m3(f, 1.0f);
+        u32x2_t w = mx_to_e4m3(f, 1.0f);
         if (!fine) w = u32x2_t{0u, 0u};
         if (c < p.kp) *(u32x2_t*)(p.q + (size_t)row * p.kp + c) = w;
       }

@@ -19,6 +19,8 @@ from . import _lib
 FORMATS = {"e2m1": 0, "e4m3": 1, "e4m3_row": 2}
 NORMS = {"rms": 0, "layer": 1}
 ACTS = {None: -1, "quick_gelu": 0, "gelu": 1}
+_BLOCKS = {"e2m1": 0, "e4m3": 1}      # formats of a product's rows
+_WEIGHTS = {"e2m1": 0}                # and of its weights
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
@@ -36,46 +38,32 @@ class MXTensor(NamedTuple):
         return self.data.shape[0], self.cols
 
 
-def _padded(cols: int) -> int:
-    return (cols + 127) // 128 * 128
+# A call on a few rows costs the host more than the GPU: the checks read each attribute once (is_cuda and get_device instead of a
+# device object), and the stream and the allocations take torch's cheaper forms (a raw stream handle, 0.1 us, instead of a Stream
+# object, 1.8; empty_strided, 1.3, instead of empty, 1.7).
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
+_empty = torch.empty_strided
 
 
-def _row_bytes(cols: int, fmt: str) -> int:
-    return _padded(cols) // 2 if fmt == "e2m1" else _padded(cols)
-
-
-# A call on a few rows costs the host more than the GPU, so the checks below read each attribute once and the stream and the
-# allocations take torch's cheaper forms (a raw stream handle instead of a Stream object, 0.1 against 1.8 us; empty_strided).
-def _stream(device: torch.device) -> int:
-    return torch._C._cuda_getCurrentRawStream(device.index)
-
-
-def _on_device(index: int):
-    """A guard for work on another device than the current one, None where it is the current one."""
-    return None if index == torch.cuda.current_device() else torch.cuda.device(index)
-
-
-def _run(device: torch.device, what: str, fn, *args) -> None:
-    """fn(*args, stream) on `device`."""
-    guard = _on_device(device.index)
-    if guard is None:
-        rc = fn(*args, _stream(device))
+def _call(index: int, what: str, fn, *args) -> None:
+    """fn(*args, stream) with device `index` current, on its current stream."""
+    if index == _current_device():
+        rc = fn(*args, _raw_stream(index))
     else:
-        with guard:
-            rc = fn(*args, _stream(device))
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
     if rc:
         _lib.check(rc, what)
 
 
 def _check_values(what: str, x: torch.Tensor, name: str = "x"):
-    """(dtype code, device, rows, cols, row stride in elements) of a matrix of values whose columns lie side by side."""
-    device = x.device
-    if device.type != "cuda":
-        raise _lib.ClipencError(f"{what} needs GPU tensors ('cuda[:i]' under PyTorch-ROCm), got {name} on {device}: this build has no CPU path")
-    dt = _DTYPES.get(x.dtype)
+    """(dtype code, device index, rows, cols, row stride in elements) of a matrix of values whose columns lie side by side."""
+    dt, shape = _DTYPES.get(x.dtype), x.shape
+    if not x.is_cuda:
+        raise _lib.ClipencError(f"{what} needs GPU tensors ('cuda[:i]' under PyTorch-ROCm), got {name} on {x.device}: this build has no CPU path")
     if dt is None:
         raise ValueError(f"{what}: {name} must be bfloat16, float16 or float32, got {x.dtype}")
-    shape = x.shape
     if len(shape) != 2 or shape[1] < 1:
         raise ValueError(f"{what}: expected {name} of shape [rows, cols], got {tuple(shape)}")
     rows, cols = shape
@@ -86,60 +74,61 @@ def _check_values(what: str, x: torch.Tensor, name: str = "x"):
         ld = cols
     elif ld < cols:
         raise ValueError(f"{what}: the rows of {name} overlap (strides {x.stride()})")
-    return dt, device, rows, cols, ld
+    return dt, x.get_device(), rows, cols, ld
 
 
 def _check_quantised(what: str, q: MXTensor, formats, name: str):
-    """(format code, device, rows, cols) of a quantised matrix."""
+    """(format code, device index, rows, cols) of a quantised matrix."""
     data, scale, fmt, cols = q
-    if fmt not in formats:
+    code = formats.get(fmt)
+    if code is None:
         raise ValueError(f"{what}: {name} must be one of {sorted(formats)}, got {fmt!r}")
     kp = (cols + 127) // 128 * 128
-    shape, device = data.shape, data.device
+    shape = data.shape
     rows = shape[0] if len(shape) == 2 else -1
-    row_bytes = kp // 2 if fmt == "e2m1" else kp
-    want, kind = ((rows,), torch.float32) if fmt == "e4m3_row" else ((rows, kp // 32), torch.uint8)
+    want, kind = ((rows, kp // 32), torch.uint8) if code != 2 else ((rows,), torch.float32)
+    row_bytes = kp if code else kp // 2
     if cols < 1 or rows < 0 or shape[1] != row_bytes or data.dtype is not torch.uint8 or scale.dtype is not kind or scale.shape != want:
         raise ValueError(f"{what}: {name} of {cols} columns in {fmt} needs uint8 data of {row_bytes} bytes a row and {kind} scales {want}, "
                          f"got {data.dtype} {tuple(shape)} and {scale.dtype} {tuple(scale.shape)}")
     if not (data.is_contiguous() and scale.is_contiguous()):
         raise ValueError(f"{what}: {name} must be contiguous")
-    if device.type != "cuda":
-        raise _lib.ClipencError(f"{what} needs GPU tensors, got {name} on {device}: this build has no CPU path")
-    if scale.device != device:
-        raise ValueError(f"{what}: the data of {name} is on {device}, its scales on {scale.device}")
-    return FORMATS[fmt], device, rows, cols
+    if not data.is_cuda:
+        raise _lib.ClipencError(f"{what} needs GPU tensors, got {name} on {data.device}: this build has no CPU path")
+    index = data.get_device()
+    if scale.get_device() != index:
+        raise ValueError(f"{what}: the data of {name} is on {data.device}, its scales on {scale.device}")
+    return code, index, rows, cols
 
 
-def _check_vector(what: str, v: Optional[torch.Tensor], n: int, device: torch.device, name: str) -> Optional[int]:
+def _check_vector(what: str, v: Optional[torch.Tensor], n: int, index: int, name: str) -> Optional[int]:
     if v is None:
         return None
     if v.dtype is not torch.float32 or v.shape != (n,) or not v.is_contiguous():
         raise ValueError(f"{what}: {name} must be a contiguous float32 [{n}], got {v.dtype} {tuple(v.shape)}")
-    if v.device != device:
-        raise ValueError(f"{what}: all tensors must be on {device}, got {name} on {v.device}")
+    if v.get_device() != index:
+        raise ValueError(f"{what}: all tensors must be on cuda:{index}, got {name} on {v.device}")
     return v.data_ptr()
-
-
-def _matrix(rows: int, cols: int, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
-    return torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=device)
 
 
 def _new(rows: int, cols: int, fmt: str, device: torch.device) -> MXTensor:
     kp = (cols + 127) // 128 * 128
-    data = _matrix(rows, kp // 2 if fmt == "e2m1" else kp, torch.uint8, device)
+    width = kp // 2 if fmt == "e2m1" else kp
+    data = _empty((rows, width), (width, 1), dtype=torch.uint8, device=device)
     if fmt == "e4m3_row":
-        return MXTensor(data, torch.empty_strided((rows,), (1,), dtype=torch.float32, device=device), fmt, cols)
-    return MXTensor(data, _matrix(rows, kp // 32, torch.uint8, device), fmt, cols)
+        return MXTensor(data, _empty((rows,), (1,), dtype=torch.float32, device=device), fmt, cols)
+    kp //= 32
+    return MXTensor(data, _empty((rows, kp), (kp, 1), dtype=torch.uint8, device=device), fmt, cols)
 
 
 def quantize(x: torch.Tensor, fmt: str = "e2m1") -> MXTensor:
     """The rows of x [rows, cols] (bf16 / fp16 / fp32, rows may be strided) in blocks of 32 columns: fmt "e2m1" or "e4m3"."""
-    if fmt != "e2m1" and fmt != "e4m3":
+    code = _BLOCKS.get(fmt)
+    if code is None:
         raise ValueError(f"quantize: fmt must be 'e2m1' or 'e4m3', got {fmt!r}")
-    dt, device, rows, cols, ld = _check_values("quantize", x)
-    q = _new(rows, cols, fmt, device)
-    _run(device, "quantize", _lib.load().clipenc_op_quant_mx, x.data_ptr(), dt, rows, cols, ld, FORMATS[fmt], q.data.data_ptr(), q.scale.data_ptr())
+    dt, index, rows, cols, ld = _check_values("quantize", x)
+    q = _new(rows, cols, fmt, x.device)
+    _call(index, "quantize", _lib.load().clipenc_op_quant_mx, x.data_ptr(), dt, rows, cols, ld, code, q[0].data_ptr(), q[1].data_ptr())
     return q
 
 
@@ -148,9 +137,10 @@ def dequantize(q: MXTensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor
     out_dt = _DTYPES.get(dtype)
     if out_dt is None:
         raise ValueError(f"dequantize: dtype must be bfloat16, float16 or float32, got {dtype}")
-    fmt, device, rows, cols = _check_quantised("dequantize", q, FORMATS, "q")
-    out = _matrix(rows, cols, dtype, device)
-    _run(device, "dequantize", _lib.load().clipenc_op_dequant_mx, q.data.data_ptr(), q.scale.data_ptr(), fmt, rows, cols, out.data_ptr(), out_dt)
+    code, index, rows, cols = _check_quantised("dequantize", q, FORMATS, "q")
+    data = q[0]
+    out = _empty((rows, cols), (cols, 1), dtype=dtype, device=data.device)
+    _call(index, "dequantize", _lib.load().clipenc_op_dequant_mx, data.data_ptr(), q[1].data_ptr(), code, rows, cols, out.data_ptr(), out_dt)
     return out
 
 
@@ -159,23 +149,26 @@ def norm_quantize(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
     """(h, q): h = x + residual (x itself without one), q = its norm ("rms" or "layer") times `weight` plus `bias`, quantised to fmt:
     "e4m3" / "e2m1" in blocks, or "e4m3_row" with one scale a row.  x, residual: [rows, cols] of one type; weight, bias: float32."""
     what = "norm_quantize"
-    if norm not in NORMS or fmt not in FORMATS:
+    kind, code = NORMS.get(norm), FORMATS.get(fmt)
+    if kind is None or code is None:
         raise ValueError(f"{what}: norm must be one of {sorted(NORMS)} and fmt one of {sorted(FORMATS)}, got {norm!r}, {fmt!r}")
-    dt, device, rows, cols, ld = _check_values(what, x)
+    dt, index, rows, cols, ld = _check_values(what, x)
+    device = x.device
     r = hp = None
     ld_r, h = 0, x
     if residual is not None:
-        if residual.shape != x.shape or residual.dtype is not x.dtype or residual.device != device:
+        dt_r, index_r, rows_r, cols_r, ld_r = _check_values(what, residual, "residual")
+        if dt_r != dt or rows_r != rows or cols_r != cols or index_r != index:
             raise ValueError(f"{what}: residual must be {x.dtype} {tuple(x.shape)} on {device}, got {residual.dtype} {tuple(residual.shape)} on {residual.device}")
-        ld_r = _check_values(what, residual, "residual")[4]
-        h = _matrix(rows, cols, x.dtype, device)
+        h = _empty((rows, cols), (cols, 1), dtype=x.dtype, device=device)
         r, hp = residual.data_ptr(), h.data_ptr()
     if weight is None:
         raise ValueError(f"{what}: weight is needed")
-    g, b = _check_vector(what, weight, cols, device, "weight"), _check_vector(what, bias, cols, device, "bias")
+    g = _check_vector(what, weight, cols, index, "weight")
+    b = None if bias is None else _check_vector(what, bias, cols, index, "bias")
     q = _new(rows, cols, fmt, device)
-    _run(device, what, _lib.load().clipenc_op_norm_quant_mx, x.data_ptr(), dt, rows, cols, ld, r, ld_r, NORMS[norm], g, b, eps, FORMATS[fmt], hp,
-         q.data.data_ptr(), q.scale.data_ptr())
+    _call(index, what, _lib.load().clipenc_op_norm_quant_mx, x.data_ptr(), dt, rows, cols, ld, r, ld_r, kind, g, b, eps, code, hp, q[0].data_ptr(),
+          q[1].data_ptr())
     return h, q
 
 
@@ -185,41 +178,47 @@ def linear(x, w: MXTensor, bias: Optional[torch.Tensor] = None, act: Optional[st
     x_fmt first; w: e2m1 [out, cols]; bias float32 [out]; act None, "quick_gelu" or "gelu" (erf), not together with a residual;
     residual [rows, out] of out_dtype (default: the values' type, bf16 for an MXTensor)."""
     what = "linear"
-    if act not in ACTS:
+    act_code = ACTS.get(act)
+    if act_code is None:
         raise ValueError(f"{what}: act must be None, 'quick_gelu' or 'gelu', got {act!r}")
-    if act is not None and residual is not None:
+    if residual is not None and act is not None:
         raise ValueError(f"{what}: activation and residual are exclusive")
-    _, device, n, w_cols = _check_quantised(what, w, ("e2m1",), "w")
+    _, index, n, w_cols = _check_quantised(what, w, _WEIGHTS, "w")
     coded = isinstance(x, MXTensor)
     if coded:
-        fmt, x_device, rows, cols = _check_quantised(what, x, ("e2m1", "e4m3"), "x")
+        fmt, x_index, rows, cols = _check_quantised(what, x, _BLOCKS, "x")
     else:
-        if x_fmt != "e2m1" and x_fmt != "e4m3":
+        fmt = _BLOCKS.get(x_fmt)
+        if fmt is None:
             raise ValueError(f"{what}: x_fmt must be 'e2m1' or 'e4m3', got {x_fmt!r}")
-        fmt = FORMATS[x_fmt]
-        dt, x_device, rows, cols, ld = _check_values(what, x)
-    if x_device != device:
-        raise ValueError(f"{what}: x is on {x_device} and w on {device}")
-    if cols != w_cols:
-        raise ValueError(f"{what}: x has {cols} columns and w {w_cols}")
+        dt, x_index, rows, cols, ld = _check_values(what, x)
+    if x_index != index or cols != w_cols:
+        raise ValueError(f"{what}: x has {cols} columns on cuda:{x_index} and w {w_cols} on cuda:{index}")
     if out_dtype is None:
         out_dtype = torch.bfloat16 if coded else x.dtype
     out_dt = _DTYPES.get(out_dtype)
     if out_dt is None:
         raise ValueError(f"{what}: out_dtype must be bfloat16, float16 or float32, got {out_dtype}")
-    b, r = _check_vector(what, bias, n, device, "bias"), None
+    b = None if bias is None else _check_vector(what, bias, n, index, "bias")
+    r = None
     if residual is not None:
-        if residual.dtype is not out_dtype or residual.shape != (rows, n) or not residual.is_contiguous() or residual.device != device:
-            raise ValueError(f"{what}: residual must be a contiguous {out_dtype} [{rows}, {n}] on {device}, got {residual.dtype} {tuple(residual.shape)} on {residual.device}")
+        if residual.dtype is not out_dtype or residual.shape != (rows, n) or not residual.is_contiguous() or residual.get_device() != index:
+            raise ValueError(f"{what}: residual must be a contiguous {out_dtype} [{rows}, {n}] on cuda:{index}, got {residual.dtype} {tuple(residual.shape)} on "
+                             f"{residual.device}")
         r = residual.data_ptr()
     lib = _lib.load()
-    out = _matrix(rows, n, out_dtype, device)
+    w_data = w[0]
+    device = w_data.device
+    out = _empty((rows, n), (n, 1), dtype=out_dtype, device=device)
     if coded:
-        _run(device, what, lib.clipenc_op_gemm_mx, x.data.data_ptr(), x.scale.data_ptr(), fmt, w.data.data_ptr(), w.scale.data_ptr(), rows, n, cols, b,
-             ACTS[act], r, out.data_ptr(), out_dt)
-    else:
-        need = lib.clipenc_op_linear_mx_ws_bytes(rows, cols, fmt)
-        ws = torch.empty_strided((need,), (1,), dtype=torch.uint8, device=device) if need else None
-        _run(device, what, lib.clipenc_op_linear_mx, x.data_ptr(), dt, ld, fmt, w.data.data_ptr(), w.scale.data_ptr(), rows, n, cols, b, ACTS[act], r,
-             out.data_ptr(), out_dt, ws.data_ptr() if need else None, need)
+        _call(index, what, lib.clipenc_op_gemm_mx, x[0].data_ptr(), x[1].data_ptr(), fmt, w_data.data_ptr(), w[1].data_ptr(), rows, n, cols, b, act_code, r,
+              out.data_ptr(), out_dt)
+        return out
+    ws = None
+    need = lib.clipenc_op_linear_mx_ws_bytes(rows, cols, fmt)
+    if need:
+        scratch = _empty((need,), (1,), dtype=torch.uint8, device=device)
+        ws = scratch.data_ptr()
+    _call(index, what, lib.clipenc_op_linear_mx, x.data_ptr(), dt, ld, fmt, w_data.data_ptr(), w[1].data_ptr(), rows, n, cols, b, act_code, r, out.data_ptr(),
+          out_dt, ws, need)
     return out
