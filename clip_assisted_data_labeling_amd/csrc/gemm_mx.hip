@@ -146,26 +146,33 @@ __device__ __forceinline__ void for_each_int(F&& f) {
   }
 }
 
-template <int AF, int BM_, int BN_, int WM_, int WN_>
+// NS: stages of A in LDS, NS - 1 of them under way.  DIRECT: scales come with each stage, a word a row and K step, and lanes read their byte
+// of it; else by periods, turned.
+template <int AF, int BM_, int BN_, int WM_, int WN_, int NS_, bool DIRECT_>
 struct Tile {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
+  static constexpr int NS = NS_, NB = NS + 1;                      // NB: biases held -- a tile may be one stage, and that many are under way
+  static constexpr bool DIRECT = DIRECT_;
   static constexpr int NW = WM * WN, THREADS = NW * 64;
   static constexpr int FM = BM / WM / 16, FN = BN / WN / 16;       // 16 x 16 fragments of a wave
   static constexpr int STEPS = AF == A_E2M1 ? 2 : 1;               // K steps of a stage of A
   static constexpr int A_BYTES = BM * 128, W_BYTES = BN * 128;
   static constexpr int A_PER = BM / 8 / NW, W_PER = BN / 8 / NW;   // DMA pieces a wave
-  static constexpr int W_OFF = 2 * A_BYTES, SC_OFF = W_OFF + 2 * W_BYTES;
-  static constexpr int SC_ROWS = BM + BN, SC_BYTES = SC_ROWS * 16, SC_PER = SC_ROWS * 4 / THREADS;
-  static constexpr int RAW_OFF = SC_OFF + 2 * SC_BYTES, BIAS_OFF = RAW_OFF + SC_BYTES, LDS = BIAS_OFF + 2 * BN * 4;
+  static constexpr int W_OFF = NS * A_BYTES, SC_OFF = W_OFF + NS * W_BYTES;
+  static constexpr int SC_ROWS = BM + BN, SC_BYTES = SC_ROWS * (DIRECT ? 4 * STEPS : 16), SC_PER = SC_ROWS * 4 / THREADS;
+  static constexpr int RAW_OFF = SC_OFF + (DIRECT ? NS : 2) * SC_BYTES, BIAS_OFF = RAW_OFF + (DIRECT ? 0 : SC_BYTES), LDS = BIAS_OFF + NB * BN * 4;
+  static constexpr int YOUNGER = (NS - 2) * (A_PER + (AF == A_E2M1 ? W_PER : 0));   // DMAs at least that are younger than the next stage's
   static constexpr int STORES = FM * FN / 2;                       // of a wave's whole 16-bit tile, 16 bytes a lane each
   static_assert(A_PER >= W_PER && FM >= 2 && FN % 2 == 0 && A_PER * NW * 8 == BM && W_PER * NW * 8 == BN && NW % 2 == 0, "pieces");
+  static_assert(BM % 64 == 0 && NS >= 2 && YOUNGER + STORES < 64, "ring");
+  static_assert(DIRECT || NS == 2, "turned scales are one stage ahead");
   static_assert(SC_PER * THREADS == SC_ROWS * 4 && BM % (THREADS / 4) == 0 && BN % 64 == 0 && BN <= THREADS, "scales, bias");
   static_assert(LDS <= 163840, "LDS");
 };
 
-template <int AF, int BM, int BN, int WM, int WN>
+template <int AF, int BM, int BN, int WM, int WN, int NS, bool DIRECT>
 __global__ __launch_bounds__(WM * WN * 64, 2) void mx_gemm_kernel(const MxGemmParams p) {
-  using T = Tile<AF, BM, BN, WM, WN>;
+  using T = Tile<AF, BM, BN, WM, WN, NS, DIRECT>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -225,6 +232,21 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mx_gemm_kernel(const MxGemmPa
       dma4(is_a ? a_at : w_at, (unsigned)min(row, (is_a ? a_rows : w_rows) - 1) * s_ld + j, lds0 + (unsigned)(T::RAW_OFF + (i * T::THREADS + w * 64) * 4));
     }
   };
+  // (DIRECT) the words of a stage's steps from K step ks on: step by step, rows of A, then of W
+  auto issue_words = [&](int m0, int n0, int ks, int buf) {
+#pragma unroll
+    for (int i = 0; i < (T::SC_ROWS * T::STEPS + T::THREADS - 1) / T::THREADS; ++i) {
+      const int at = i * T::THREADS + w * 64;                       // the wave's first word
+      if (at >= T::SC_ROWS * T::STEPS) break;
+      const int step = at / T::SC_ROWS, row = at % T::SC_ROWS;
+      const bool is_a = row < BM;
+      const int r = row - (is_a ? 0 : BM) + lane;
+      const int dst = T::SC_OFF + buf * T::SC_BYTES + at * 4;
+      if (ks + step < 0) { *(uint32_t*)(smem + dst + lane * 4) = 0u; continue; }     // the empty step
+      const uint8_t* base = uniform(is_a ? p.a_scale + (long)m0 * s_ld : p.w_scale + (long)n0 * s_ld) + (ks + step) * 4;
+      dma4(base, (unsigned)min(r, (is_a ? p.M - m0 : p.N - n0) - 1) * s_ld, lds0 + (unsigned)dst);
+    }
+  };
   const uint32_t sc_sel = 0x01010101u * (uint32_t)(tid & 3) + 0x00000400u;      // bytes (own, own + 4) of a register pair
   auto turn_scales = [&](int period, int buf) {
     const uint32_t keep = AF == A_E2M1 && odd && period == 0 && (tid & 3) == 0 ? 0u : 0xffffffffu;   // the empty step's word
@@ -256,8 +278,11 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mx_gemm_kernel(const MxGemmPa
       return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1);
     }
   };
-  auto load_scale = [&](int sbuf, int in_period, int row16) -> uint32_t {   // the stage's one or two bytes of the lane's word
-    const char* at = smem + T::SC_OFF + sbuf * T::SC_BYTES + r16 * 16 + g * 4 + row16 * 256 + in_period;
+  // (turned) the one or two bytes of a stage in the lane's word of the period;  (DIRECT) the byte of the stage's step
+  auto load_scale = [&](int sbuf, int in_period, int step, int row16) -> uint32_t {
+    const char* at = smem + T::SC_OFF + sbuf * T::SC_BYTES;
+    if constexpr (DIRECT) return *(const uint8_t*)(at + (step * T::SC_ROWS + row16 * 16 + r16) * 4 + g);
+    at += r16 * 16 + g * 4 + row16 * 256 + in_period;
     return T::STEPS == 2 ? (uint32_t)*(const uint16_t*)at : (uint32_t)*(const uint8_t*)at;
   };
   constexpr int FM = T::FM, FN = T::FN, N = T::STEPS * FM;          // N row fragments a stage
@@ -265,6 +290,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mx_gemm_kernel(const MxGemmPa
   // The stage to ask for next (f_): where its rows begin, its buffers, and which period it opens, whose scales are then to be turned
   const int v0 = AF == A_E2M1 ? 0 : odd;           // a tile's first stage's step (of e4m3 rows the empty step is no stage)
   int f_idx = blockIdx.x, f_v = v0, f_ab = 0, f_wb = 0, f_bias = 0, f_period = -1, f_m0, f_n0;
+  auto after = [](int buf, int of) { return buf + 1 == of ? 0 : buf + 1; };
   const uint8_t *f_a, *f_w, *f_sa, *f_sw;
   auto fetch_tile = [&]() {
     tile_at(f_idx, f_m0, f_n0);
@@ -282,14 +308,15 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mx_gemm_kernel(const MxGemmPa
     issue(f_a, a_off, a_hop, (unsigned)(p.M - 1 - f_m0) * a_ld, f_m0 + BM <= p.M, AF == A_E2M1 && first && odd, std::integral_constant<int, T::A_PER>{},
           lds0 + (unsigned)(f_ab * T::A_BYTES + w * 1024));
     f_a += 128;
-    f_ab ^= 1;
+    if constexpr (DIRECT) issue_words(f_m0, f_n0, f_v - odd, f_ab);
+    f_ab = after(f_ab, NS);
     if (AF == A_E2M1 || (f_v & 1) == 0 || first) {
       issue(f_w, w_off, w_hop, (unsigned)(p.N - 1 - f_n0) * w_ld, f_n0 + BN <= p.N, first && odd, std::integral_constant<int, T::W_PER>{},
             lds0 + (unsigned)(T::W_OFF + f_wb * T::W_BYTES + w * 1024));
       f_w += 128;
-      f_wb ^= 1;
+      f_wb = after(f_wb, NS);
     }
-    if ((f_v & 3) == 0 || first) {
+    if (!DIRECT && ((f_v & 3) == 0 || first)) {
       f_period = f_v >> 2;
       issue_scales(f_sa, f_sw, p.M - f_m0, p.N - f_n0, f_period);
       f_sa += 16;
@@ -298,7 +325,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mx_gemm_kernel(const MxGemmPa
     if (first) {
       if (p.bias && w < BN / 64)
         dma4((const uint8_t*)p.bias, (unsigned)min(f_n0 + tid, p.N - 1) * 4u, lds0 + (unsigned)(T::BIAS_OFF + f_bias * BN * 4 + w * 256));
-      f_bias ^= 1;
+      f_bias = after(f_bias, T::NB);
     }
     f_v += T::STEPS;
     if (f_v >= steps) {
@@ -310,23 +337,33 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mx_gemm_kernel(const MxGemmPa
   int idx = blockIdx.x, m0, n0;
   tile_at(idx, m0, n0);
   int ab = 0, wb = 0, sb = 0, bias_buf = 0;        // the buffers of the current stage, of the current tile's bias
-  fetch();
-  WAIT_ALL();
-  turn_scales(0, 0);
-  WAIT_ALL();
+  // What was asked for NS - 1 stages ago has to be there; younger are the stages since then (in the order of the asking), and a finished
+  // tile's results, which need not have left.
+  auto wait_stage = [&](bool stored) {
+    const bool more = f_idx < nwg;                 // else fewer stages are younger
+    if (NS > 2 && more && stored) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "i"(T::YOUNGER + T::STORES) : "memory");
+    else if (NS > 2 && more) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "i"(T::YOUNGER) : "memory");
+    else if (stored) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "i"(T::STORES) : "memory");
+    else WAIT_ALL();
+  };
+#pragma unroll
+  for (int i = 0; i < NS - 1; ++i) fetch();
+  wait_stage(false);
+  if (!DIRECT) turn_scales(0, 0);
+  WAIT_LDS();
   BARRIER();
   fetch();
   i32x8_t wf[2][FN], af[3];
-  uint32_t sa[3], sw[FN];
+  uint32_t sa[3], sw[FN], sw1[FN];               // sw1 (DIRECT): of the second step
   auto first_fragments = [&](int in_period, i32x8_t (&w_)[FN], i32x8_t& a0, i32x8_t& a1, uint32_t (&sw_)[FN], uint32_t& s0, uint32_t& s1) {
 #pragma unroll
     for (int j = 0; j < FN; ++j) w_[j] = load_w(wb, in_period, 0, j);
     a0 = load_a(ab, 0, 0);
 #pragma unroll
-    for (int j = 0; j < FN; ++j) sw_[j] = load_scale(sb, in_period, FM * WM + wn * FN + j);
-    s0 = load_scale(sb, in_period, wm * FM);
+    for (int j = 0; j < FN; ++j) sw_[j] = load_scale(sb, in_period, 0, FM * WM + wn * FN + j);
+    s0 = load_scale(sb, in_period, 0, wm * FM);
     a1 = load_a(ab, 0, 1);
-    s1 = load_scale(sb, in_period, wm * FM + 1);
+    s1 = load_scale(sb, in_period, 0, wm * FM + 1);
   };
   bool stored = false;                             // the previous tile's STORES stores may still be on their way, issued after the loads
   while (true) {
@@ -344,26 +381,30 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mx_gemm_kernel(const MxGemmPa
         __builtin_amdgcn_sched_barrier(0);
         i32x8_t a = af[t % 3];
         const int s = (int)sa[t % 3];
+        constexpr int OP = DIRECT ? 0 : step;
         if constexpr (AF == A_E4M3_BANDS) {
           const i32x8_t high = high_band(a);
           a ^= high;
 #pragma unroll
           for (int j = 0; j < FN; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[step][j], high, acc[i][j], 4, 0, step, (int)sw[j], step, s);
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[step][j], high, acc[i][j], 4, 0, OP, (int)(DIRECT && step ? sw1[j] : sw[j]), OP, s);
         }
 #pragma unroll
         for (int j = 0; j < FN; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[step][j], a, acc[i][j], 4, AF != A_E2M1 ? 0 : 4, step, (int)sw[j], step, s);
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[step][j], a, acc[i][j], 4, AF != A_E2M1 ? 0 : 4, OP, (int)(DIRECT && step ? sw1[j] : sw[j]), OP, s);
         __builtin_amdgcn_sched_barrier(0);
       };
       for_each_int<0, N - 2>([&](auto t_) {
         constexpr int t = decltype(t_)::value, step = t / FM, i = t % FM;
         af[(t + 2) % 3] = load_a(ab, (t + 2) / FM, (t + 2) % FM);
-        sa[(t + 2) % 3] = load_scale(sb, v & 3, wm * FM + (t + 2) % FM);
+        sa[(t + 2) % 3] = load_scale(sb, v & 3, (t + 2) / FM, wm * FM + (t + 2) % FM);
         if constexpr (step + 1 < T::STEPS) {
 #pragma unroll
           for (int j = 0; j < FN; ++j)
-            if (FM - FN + j == i || (FM < FN && i == 0)) wf[1][j] = load_w(wb, 0, 1, j);
+            if (FM - FN + j == i || (FM < FN && i == 0)) {
+              wf[1][j] = load_w(wb, 0, 1, j);
+              if constexpr (DIRECT) sw1[j] = load_scale(sb, 0, 1, FM * WM + wn * FN + j);
+            }
         }
         products(t_);
       });
@@ -371,19 +412,18 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mx_gemm_kernel(const MxGemmPa
       for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int j = 0; j < FN; ++j) asm volatile("" : "+v"(acc[i][j]));       // the products stay in front of the wait (no instruction)
-      // All of the stage is in registers.  What was asked for a stage ago is the next stage; younger than it are only a finished tile's
-      // results, which need not have left.
-      if (stored) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "i"(T::STORES) : "memory");
-      else WAIT_ALL();
+      // All of the stage is in registers.
+      wait_stage(stored);
       stored = false;
       last = v + T::STEPS >= steps;
       const int next_v = last ? v0 : v + T::STEPS;
-      if (f_period >= 0) turn_scales(f_period, sb ^ 1);
+      if (!DIRECT && f_period >= 0) turn_scales(f_period, sb ^ 1);
       WAIT_LDS();
       BARRIER();
-      ab ^= 1;
-      if (AF == A_E2M1 || (next_v & 1) == 0 || last) wb ^= 1;
-      if ((next_v & 3) == 0 || last) sb ^= 1;
+      ab = after(ab, NS);
+      if (AF == A_E2M1 || (next_v & 1) == 0 || last) wb = after(wb, NS);
+      if (DIRECT) sb = ab;
+      else if ((next_v & 3) == 0 || last) sb ^= 1;
       i32x8_t w_next[FN], a0, a1;
       uint32_t sw_next[FN], s0, s1;
       first_fragments(next_v & 3, w_next, a0, a1, sw_next, s0, s1);
@@ -473,7 +513,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mx_gemm_kernel(const MxGemmPa
         __builtin_amdgcn_sched_barrier(0);
       }
     }
-    bias_buf ^= 1;
+    bias_buf = after(bias_buf, T::NB);
     idx += (int)gridDim.x;
     if (idx >= nwg) break;
     tile_at(idx, m0, n0);
@@ -554,8 +594,18 @@ __device__ __forceinline__ void load16(const T* row, int c, int k, float* v) {
 
 constexpr int FEW_WAVES = 8;
 
-// T = void: the rows are quantised;  AF: A_*;  MF: 16-row fragments
-template <typename T, int AF, int MF>
+// Scale words of U neighbouring K steps of a row, the lane's byte lowest
+template <int U>
+__device__ __forceinline__ void load_words(const uint8_t* scales, size_t step, int g, uint32_t (&s)[U]) {
+  struct __attribute__((packed, aligned(4))) Words { uint32_t v[U]; };
+  const Words w = *(const Words*)(scales + step * 4);
+#pragma unroll
+  for (int u = 0; u < U; ++u) s[u] = w.v[u] >> (8 * g);
+}
+
+// T = void: the rows are quantised;  AF: A_*;  MF: 16-row fragments;  U: K steps whose loads are under way together.  A wave has
+// neighbouring steps, so that it reads whole lines of its rows and the scales of U steps at once.
+template <typename T, int AF, int MF, int U>
 __global__ __launch_bounds__(FEW_WAVES * 64) void mx_few_kernel(const MxFewParams fp) {
   const MxGemmParams& p = fp.g;
   constexpr bool VALUES = !std::is_same<T, void>::value;
@@ -565,61 +615,62 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void mx_few_kernel(const MxFewParam
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6), waves = blockDim.x >> 6;
   const int n0 = blockIdx.x * 16, m0 = blockIdx.y * (MF * 16);
   const size_t w_row = (size_t)min(n0 + r16, p.N - 1) * p.nk;                      // in K steps
+  size_t a_row[MF];
+#pragma unroll
+  for (int i = 0; i < MF; ++i) a_row[i] = (size_t)min(m0 + i * 16 + r16, p.M - 1) * (VALUES ? (size_t)fp.ld_x : (size_t)p.nk);
   f32x4_t acc[MF];
 #pragma unroll
   for (int i = 0; i < MF; ++i) acc[i] = f32x4_t{0, 0, 0, 0};
-  constexpr int U = VALUES ? 2 : MF == 1 ? 4 : 2;                                  // K steps in flight
-  for (int ks0 = w; ks0 < p.nk; ks0 += U * waves) {
-    i32x8_t wf[U], af[U][MF];
-    uint32_t sw[U], sa[U][MF];
+  auto steps = [&](int ks, auto n_) {
+    constexpr int C = decltype(n_)::value;
+    i32x8_t wf[C], af[C][MF];
+    uint32_t sw[C], sa[MF][C];
+    load_words<C>(p.w_scale, w_row + ks, g, sw);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int ks = min(ks0 + u * waves, p.nk - 1);                               // (behind the end: that step again, not multiplied)
-      const i32x4_t v = *(const i32x4_t*)(p.w + (w_row + ks) * 64 + g * 16);
+    for (int i = 0; i < MF; ++i)
+      if constexpr (!VALUES) load_words<C>(p.a_scale, a_row[i] + ks, g, sa[i]);
+#pragma unroll
+    for (int u = 0; u < C; ++u) {
+      const i32x4_t v = *(const i32x4_t*)(p.w + (w_row + ks + u) * 64 + g * 16);
       wf[u] = __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1);
-      sw[u] = p.w_scale[(w_row + ks) * 4 + g];
 #pragma unroll
       for (int i = 0; i < MF; ++i) {
-        const size_t row = (size_t)min(m0 + i * 16 + r16, p.M - 1);
         if constexpr (VALUES) {
-          const T* x = (const T*)fp.x + row * fp.ld_x;
+          const T* x = (const T*)fp.x + a_row[i];
+          const int c = (ks + u) * 128 + g * (FMT == MX_E2M1 ? 32 : 16);
           float f[32];
-          if (FMT == MX_E2M1) {
-            load16(x, ks * 128 + g * 32, fp.k, f);
-            load16(x, ks * 128 + g * 32 + 16, fp.k, f + 16);
-          } else {
-            load16(x, ks * 128 + g * 16, fp.k, f);
-            load16(x, ks * 128 + 64 + g * 16, fp.k, f + 16);
-          }
-          af[u][i] = quantise_fragment(f, FMT, sa[u][i]);
+          load16(x, c, fp.k, f);
+          load16(x, c + (FMT == MX_E2M1 ? 16 : 64), fp.k, f + 16);
+          af[u][i] = quantise_fragment(f, FMT, sa[i][u]);
+        } else if constexpr (AF == A_E2M1) {
+          const i32x4_t q = *(const i32x4_t*)(p.a + (a_row[i] + ks + u) * 64 + g * 16);
+          af[u][i] = __builtin_shufflevector(q, q, 0, 1, 2, 3, -1, -1, -1, -1);
         } else {
-          sa[u][i] = p.a_scale[(row * p.nk + ks) * 4 + g];
-          if constexpr (AF == A_E2M1) {
-            const i32x4_t q = *(const i32x4_t*)(p.a + (row * p.nk + ks) * 64 + g * 16);
-            af[u][i] = __builtin_shufflevector(q, q, 0, 1, 2, 3, -1, -1, -1, -1);
-          } else {
-            const uint8_t* q = p.a + (row * p.nk + ks) * 128 + g * 16;
-            const i32x4_t lo = *(const i32x4_t*)q, hi = *(const i32x4_t*)(q + 64);
-            af[u][i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-          }
+          const uint8_t* q = p.a + (a_row[i] + ks + u) * 128 + g * 16;
+          const i32x4_t lo = *(const i32x4_t*)q, hi = *(const i32x4_t*)(q + 64);
+          af[u][i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
         }
       }
     }
+    __builtin_amdgcn_sched_barrier(0);                                             // the loads in front of the products
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (ks0 + u * waves >= p.nk) break;                                          // (the same for the whole wave)
+    for (int u = 0; u < C; ++u)
 #pragma unroll
       for (int i = 0; i < MF; ++i) {
         i32x8_t a = af[u][i];
         if constexpr (AF == A_E4M3_BANDS) {
           const i32x8_t high = high_band(a);
           a ^= high;
-          acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[u], high, acc[i], 4, 0, 0, (int)sw[u], 0, (int)sa[u][i]);
+          acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[u], high, acc[i], 4, 0, 0, (int)sw[u], 0, (int)sa[i][u]);
         }
-        acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[u], a, acc[i], 4, AF != A_E2M1 ? 0 : 4, 0, (int)sw[u], 0, (int)sa[u][i]);
+        acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[u], a, acc[i], 4, AF != A_E2M1 ? 0 : 4, 0, (int)sw[u], 0, (int)sa[i][u]);
       }
-    }
-  }
+  };
+  const int per = (p.nk + waves - 1) / waves, end = min((w + 1) * per, p.nk);
+  int ks = w * per;
+  for (; ks + U <= end; ks += U) steps(ks, std::integral_constant<int, U>{});
+  if constexpr (U > 1)
+    for (; ks < end; ++ks) steps(ks, std::integral_constant<int, 1>{});
 #pragma unroll
   for (int i = 0; i < MF; ++i) *(f32x4_t*)&sums[w][i][r16 * 16 + g * 4] = acc[i];   // row r16, columns 4 g .. 4 g + 3
   __syncthreads();
@@ -637,25 +688,46 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void mx_few_kernel(const MxFewParam
   }
 }
 
-template <typename T, int AF, int MF>
-hipError_t launch_few(const MxFewParams& p, hipStream_t stream) {
+template <typename T, int AF, int MF, int U>
+hipError_t launch_few_u(const MxFewParams& p, hipStream_t stream) {
   const int waves = p.g.nk < FEW_WAVES ? p.g.nk : FEW_WAVES;
-  hipLaunchKernelGGL((mx_few_kernel<T, AF, MF>), dim3((unsigned)((p.g.N + 15) / 16), (unsigned)((p.g.M + MF * 16 - 1) / (MF * 16))), dim3((unsigned)waves * 64), 0,
+  hipLaunchKernelGGL((mx_few_kernel<T, AF, MF, U>), dim3((unsigned)((p.g.N + 15) / 16), (unsigned)((p.g.M + MF * 16 - 1) / (MF * 16))), dim3((unsigned)waves * 64), 0,
                      stream, p);
   return hipGetLastError();
 }
+// as many steps under way as a wave has, and its registers hold
+template <typename T, int AF, int MF>
+hipError_t launch_few(const MxFewParams& p, hipStream_t stream) {
+  const int per = (p.g.nk + FEW_WAVES - 1) / FEW_WAVES;
+  if constexpr (std::is_same<T, void>::value && MF <= 2)
+    if (per >= 4) return launch_few_u<T, AF, MF, 4>(p, stream);
+  return per >= 2 ? launch_few_u<T, AF, MF, 2>(p, stream) : launch_few_u<T, AF, MF, 1>(p, stream);
+}
 
-template <int AF, int BM, int BN, int WM, int WN>
+template <int AF, int BM, int BN, int WM, int WN, int NS, bool DIRECT>
 hipError_t launch(const MxGemmParams& p, hipStream_t stream) {
-  using T = Tile<AF, BM, BN, WM, WN>;
+  using T = Tile<AF, BM, BN, WM, WN, NS, DIRECT>;
   static DeviceKernelSetup setup;
   int n_cu = 0;
-  if (hipError_t e = setup.ensure((const void*)mx_gemm_kernel<AF, BM, BN, WM, WN>, T::LDS, &n_cu); e != hipSuccess) return e;
+  if (hipError_t e = setup.ensure((const void*)mx_gemm_kernel<AF, BM, BN, WM, WN, NS, DIRECT>, T::LDS, &n_cu); e != hipSuccess) return e;
   const long tiles = (long)((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN);
   if (tiles > 0x3fffffff) return hipErrorInvalidValue;
   const long resident = (long)n_cu * (163840 / T::LDS);             // workgroups that the CUs hold
-  hipLaunchKernelGGL((mx_gemm_kernel<AF, BM, BN, WM, WN>), dim3((unsigned)(tiles < resident ? tiles : resident)), dim3(T::THREADS), T::LDS, stream, p);
+  hipLaunchKernelGGL((mx_gemm_kernel<AF, BM, BN, WM, WN, NS, DIRECT>), dim3((unsigned)(tiles < resident ? tiles : resident)), dim3(T::THREADS), T::LDS, stream, p);
   return hipGetLastError();
+}
+
+// Fewer than a 256 x 256 tile a CU.  64 x 64 tiles while the CUs hold them in one go or nearly (two a CU, a third one joins late); beyond that
+// 128 x 128: 5120 columns of 577 / 1154 rows, e4m3: 19 / 25 us in 64 x 64, 15 / 17 in 128 x 128 -- in eight waves with four stages in LDS while
+// they are at most one a CU, and latency is what a stage costs, else in four waves, two workgroups a CU.  (e4m3 in bands: waves of 32 x 64, which
+// part each row fragment for four products instead of two: 46 -> 40 us at 2885 x 4001 -> 1003.)
+template <int AF>
+hipError_t small_tiles(const MxGemmParams& p, hipStream_t stream) {
+  const long tiles64 = (long)((p.M + 63) / 64) * ((p.N + 63) / 64), tiles128 = (long)((p.M + 127) / 128) * ((p.N + 127) / 128);
+  if (tiles64 <= 704) return launch<AF, 64, 64, 2, 2, 4, true>(p, stream);
+  if (tiles128 > 256) return launch<AF, 128, 128, 2, 2, 2, false>(p, stream);
+  if constexpr (AF == A_E4M3_BANDS) return launch<AF, 128, 128, 4, 2, 4, true>(p, stream);
+  else return launch<AF, 128, 128, 2, 4, 4, true>(p, stream);
 }
 
 template <int AF>
@@ -669,20 +741,20 @@ hipError_t choose(MxGemmParams p, hipStream_t stream) {
   // leave three quarters of the CUs idle, its rows go to a second launch in small tiles: 65 792 x 4096 -> 1024 is 4 rounds and 4 tiles.
   constexpr int CUS = 256;
   const long tn = (p.N + 255) / 256, tiles = (long)((p.M + 255) / 256) * tn;
-  if (tiles < CUS) return launch<AF, 64, 64, 2, 2>(p, stream);
+  if (tiles < CUS) return small_tiles<AF>(p, stream);
   const int rest = (int)(tiles % CUS);
   const long rows = tiles / CUS * CUS / tn * 256;
-  if (rest == 0 || rest * 4 > CUS || rows == 0 || rows >= p.M) return launch<AF, 256, 256, 2, 4>(p, stream);
+  if (rest == 0 || rest * 4 > CUS || rows == 0 || rows >= p.M) return launch<AF, 256, 256, 2, 4, 2, false>(p, stream);
   const int M = p.M;
   p.M = (int)rows;
-  if (hipError_t e = launch<AF, 256, 256, 2, 4>(p, stream); e != hipSuccess) return e;
+  if (hipError_t e = launch<AF, 256, 256, 2, 4, 2, false>(p, stream); e != hipSuccess) return e;
   p.M = M - (int)rows;
   p.a += (size_t)rows * p.nk * (AF == A_E2M1 ? 64 : 128);
   p.a_scale += (size_t)rows * p.nk * 4;
   const size_t skip = (size_t)rows * p.N * (p.out_dtype == MX_DT_F32 ? 4 : 2);
   p.out = (char*)p.out + skip;
   if (p.resid) p.resid = (const char*)p.resid + skip;
-  return launch<AF, 64, 64, 2, 2>(p, stream);
+  return small_tiles<AF>(p, stream);
 }
 
 }  // namespace

@@ -268,6 +268,28 @@ def test_linear_of_many_rows(gpu, m, n, k, fmt):
 
 
 @pytest.mark.parametrize("fmt", ["e2m1", "e4m3"])
+@pytest.mark.parametrize("m,n,k", [(2900, 3001, 100), (2900, 3001, 200), (2900, 3001, 300), (2900, 3001, 700), (2885, 1003, 600), (5800, 3001, 100), (16700, 4100, 100), (16700, 4100, 300)])
+def test_linear_of_more_tiles_than_the_gpu_holds(gpu, m, n, k, fmt):
+    """Workgroups that walk several tiles of one, two or three stages; every row and column has its own bias and residual."""
+    a, av = _random_coded(m, k, fmt, 1, gpu)
+    w, wv = _random_coded(n, k, "e2m1", 2, gpu)
+    a, av = mx.MXTensor(a.data, a.scale - 8, fmt, k), av * 2.0 ** -8
+    g = torch.Generator().manual_seed(k)
+    bias, res = torch.randn(n, generator=g) * 100, (torch.randn(m, n, generator=g) * 100).to(torch.bfloat16)
+    aa, ww = torch.from_numpy(av).to(gpu), torch.from_numpy(wv).to(gpu)
+    size = aa.abs() @ ww.abs().t().contiguous()
+    u = aa @ ww.t().contiguous() + bias.to(gpu).double()
+    cut = torch.from_numpy(np.asarray(_linear_cut(a, w, torch.bfloat16))).to(gpu)
+    pre = (128 + ora.padded(k) // 128 + 2) * U * (size + bias.to(gpu).double().abs()) + cut
+    for _ in range(3):
+        y = mx.linear(a, w, bias=bias.to(gpu), residual=res.to(gpu))
+        want = u + res.to(gpu).double()
+        assert ((y.double() - want).abs() <= pre + 2 * U * want.abs() + 2.0 ** -8 * (want.abs() + pre)).all()
+        y = mx.linear(a, w, bias=bias.to(gpu))
+        assert ((y.double() - u).abs() <= pre + 2 * U * u.abs() + 2.0 ** -8 * (u.abs() + pre)).all()
+
+
+@pytest.mark.parametrize("fmt", ["e2m1", "e4m3"])
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("m,n,k", [(1, 1664, 1280), (1, 33, 77), (7, 500, 300), (16, 256, 2048), (17, 128, 640), (40, 200, 4096), (64, 320, 1001), (65, 96, 512), (300, 130, 200)])
 def test_linear_of_values_is_quantize_and_linear(gpu, m, n, k, dtype, fmt):
