@@ -67,7 +67,7 @@ __device__ __forceinline__ void dma16(const uint8_t* base, unsigned off, unsigne
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(base), "s"(lds_addr) : "memory");
 }
 __device__ __forceinline__ void dma4(const uint8_t* base, unsigned off, unsigned lds_addr) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" : : "v"(off), "s"(base), "s"(lds_addr) : "memory");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" : : "v"(off), "s"(base), "s"(__builtin_amdgcn_readfirstlane(lds_addr)) : "memory");
 }
 #define WAIT_LDS() asm volatile("s_waitcnt lgkmcnt(0)" : : : "memory")
 #define WAIT_ALL() asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" : : : "memory")
@@ -147,8 +147,8 @@ __device__ __forceinline__ void for_each_int(F&& f) {
 }
 
 // NS: stages of A in LDS, NS - 1 of them under way.  DIRECT: scales come with each stage, a word a row and K step, and lanes read their byte
-// of it; else by periods, turned.
-template <int AF, int BM_, int BN_, int WM_, int WN_, int NS_, bool DIRECT_>
+// of it; else by periods, turned.  PAIRED: the two rows of waves in turns.
+template <int AF, int BM_, int BN_, int WM_, int WN_, int NS_, bool DIRECT_, bool PAIRED_>
 struct Tile {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
   static constexpr int NS = NS_, NB = NS + 1;                      // NB: biases held -- a tile may be one stage, and that many are under way
@@ -166,13 +166,14 @@ struct Tile {
   static_assert(A_PER >= W_PER && FM >= 2 && FN % 2 == 0 && A_PER * NW * 8 == BM && W_PER * NW * 8 == BN && NW % 2 == 0, "pieces");
   static_assert(BM % 64 == 0 && NS >= 2 && YOUNGER + STORES < 64, "ring");
   static_assert(DIRECT || NS == 2, "turned scales are one stage ahead");
+  static_assert(!PAIRED_ || (AF == A_E4M3 && !DIRECT && WM == 2 && BM == BN && BN / 64 == WN && WN % 2 == 0), "turns");
   static_assert(SC_PER * THREADS == SC_ROWS * 4 && BM % (THREADS / 4) == 0 && BN % 64 == 0 && BN <= THREADS, "scales, bias");
   static_assert(LDS <= 163840, "LDS");
 };
 
-template <int AF, int BM, int BN, int WM, int WN, int NS, bool DIRECT>
+template <int AF, int BM, int BN, int WM, int WN, int NS, bool DIRECT, bool PAIRED = false>
 __global__ __launch_bounds__(WM * WN * 64, 2) void mx_gemm_kernel(const MxGemmParams p) {
-  using T = Tile<AF, BM, BN, WM, WN, NS, DIRECT>;
+  using T = Tile<AF, BM, BN, WM, WN, NS, DIRECT, PAIRED>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -183,7 +184,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mx_gemm_kernel(const MxGemmPa
   // tile i of the walk: neighbouring workgroups of one XCD (i mod 8) walk neighbouring tiles, 8 row tiles deep
   const int tiles_m = (p.M + BM - 1) / BM, tiles_n = (p.N + BN - 1) / BN;
   const int nwg = tiles_m * tiles_n;
-  auto tile_at = [&](int i, int& m0, int& n0) {
+  auto tile_at = [&](int i, int& m0, int& n0) __attribute__((always_inline)) {
     const int q = nwg >> 3, rem = nwg & 7, xcd = i & 7, pos = i >> 3;
     const int bid = (xcd < rem ? xcd * (q + 1) : rem * (q + 1) + (xcd - rem) * q) + pos;
     constexpr int GM = 8;
@@ -220,7 +221,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mx_gemm_kernel(const MxGemmPa
   // brought -- and leaves its word where the fragments' lanes read it.
   const unsigned s_ld = (unsigned)p.nk * 4u;
   const int periods = (steps + 3) >> 2;
-  auto issue_scales = [&](const uint8_t* a_at, const uint8_t* w_at, int a_rows, int w_rows, int period) {
+  auto issue_scales = [&](const uint8_t* a_at, const uint8_t* w_at, int a_rows, int w_rows, int period) __attribute__((always_inline)) {
     // (a_at, w_at: where the period's words of the tile's first rows would begin)
     unsigned j = (unsigned)(tid & 3) * 4u;
     if (period == 0 && odd) j = max(j, 4u);
@@ -248,7 +249,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mx_gemm_kernel(const MxGemmPa
     }
   };
   const uint32_t sc_sel = 0x01010101u * (uint32_t)(tid & 3) + 0x00000400u;      // bytes (own, own + 4) of a register pair
-  auto turn_scales = [&](int period, int buf) {
+  auto turn_scales = [&](int period, int buf) __attribute__((always_inline)) {
     const uint32_t keep = AF == A_E2M1 && odd && period == 0 && (tid & 3) == 0 ? 0u : 0xffffffffu;   // the empty step's word
 #pragma unroll
     for (int i = 0; i < T::SC_PER; ++i) {
@@ -263,12 +264,12 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mx_gemm_kernel(const MxGemmPa
   f32x4_t acc[T::FM][T::FN];
   const int rd = (r16 >> 3) * 1024 + (r16 & 7) * 128 + ((g ^ ((r16 >> 1) & 7)) << 4);   // chunk g of row r16; chunk g + 4: ^ 64
   // Fragments of a stage whose first K step is number `in_period` (0 .. 3) of its period
-  auto load_w = [&](int wbuf, int in_period, int step, int j) {
+  auto load_w = [&](int wbuf, int in_period, int step, int j) __attribute__((always_inline)) {
     const int at = AF == A_E2M1 ? rd : rd ^ ((in_period & 1) * 64);
     const i32x4_t v = *(const i32x4_t*)(smem + T::W_OFF + wbuf * T::W_BYTES + (wn * T::FN + j) * 2048 + (at ^ (step * 64)));
     return __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1);
   };
-  auto load_a = [&](int abuf, int step, int i) {
+  auto load_a = [&](int abuf, int step, int i) __attribute__((always_inline)) {
     const char* at = smem + abuf * T::A_BYTES + (wm * T::FM + i) * 2048;
     if constexpr (AF != A_E2M1) {
       const i32x4_t lo = *(const i32x4_t*)(at + rd), hi = *(const i32x4_t*)(at + (rd ^ 64));
@@ -279,7 +280,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mx_gemm_kernel(const MxGemmPa
     }
   };
   // (turned) the one or two bytes of a stage in the lane's word of the period;  (DIRECT) the byte of the stage's step
-  auto load_scale = [&](int sbuf, int in_period, int step, int row16) -> uint32_t {
+  auto load_scale = [&](int sbuf, int in_period, int step, int row16) __attribute__((always_inline)) -> uint32_t {
     const char* at = smem + T::SC_OFF + sbuf * T::SC_BYTES;
     if constexpr (DIRECT) return *(const uint8_t*)(at + (step * T::SC_ROWS + row16 * 16 + r16) * 4 + g);
     at += r16 * 16 + g * 4 + row16 * 256 + in_period;
@@ -290,7 +291,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mx_gemm_kernel(const MxGemmPa
   // The stage to ask for next (f_): where its rows begin, its buffers, and which period it opens, whose scales are then to be turned
   const int v0 = AF == A_E2M1 ? 0 : odd;           // a tile's first stage's step (of e4m3 rows the empty step is no stage)
   int f_idx = blockIdx.x, f_v = v0, f_ab = 0, f_wb = 0, f_bias = 0, f_period = -1, f_m0, f_n0;
-  auto after = [](int buf, int of) { return buf + 1 == of ? 0 : buf + 1; };
+  auto after = [](int buf, int of) __attribute__((always_inline)) { return buf + 1 == of ? 0 : buf + 1; };
   const uint8_t *f_a, *f_w, *f_sa, *f_sw;
   auto fetch_tile = [&]() {
     tile_at(f_idx, f_m0, f_n0);
@@ -300,7 +301,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mx_gemm_kernel(const MxGemmPa
     f_sa = uniform(p.a_scale + ((long)f_m0 * s_ld - odd * 4));
     f_sw = uniform(p.w_scale + ((long)f_n0 * s_ld - odd * 4));
   };
-  fetch_tile();
+  if constexpr (!PAIRED) fetch_tile();
   auto fetch = [&]() {
     f_period = -1;
     if (f_idx >= nwg) return;
@@ -339,107 +340,17 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mx_gemm_kernel(const MxGemmPa
   int ab = 0, wb = 0, sb = 0, bias_buf = 0;        // the buffers of the current stage, of the current tile's bias
   // What was asked for NS - 1 stages ago has to be there; younger are the stages since then (in the order of the asking), and a finished
   // tile's results, which need not have left.
-  auto wait_stage = [&](bool stored) {
+  auto wait_stage = [&](bool stored) __attribute__((always_inline)) {
     const bool more = f_idx < nwg;                 // else fewer stages are younger
     if (NS > 2 && more && stored) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "i"(T::YOUNGER + T::STORES) : "memory");
     else if (NS > 2 && more) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "i"(T::YOUNGER) : "memory");
     else if (stored) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "i"(T::STORES) : "memory");
     else WAIT_ALL();
   };
-#pragma unroll
-  for (int i = 0; i < NS - 1; ++i) fetch();
-  wait_stage(false);
-  if (!DIRECT) turn_scales(0, 0);
-  WAIT_LDS();
-  BARRIER();
-  fetch();
-  i32x8_t wf[2][FN], af[3];
-  uint32_t sa[3], sw[FN], sw1[FN];               // sw1 (DIRECT): of the second step
-  auto first_fragments = [&](int in_period, i32x8_t (&w_)[FN], i32x8_t& a0, i32x8_t& a1, uint32_t (&sw_)[FN], uint32_t& s0, uint32_t& s1) {
-#pragma unroll
-    for (int j = 0; j < FN; ++j) w_[j] = load_w(wb, in_period, 0, j);
-    a0 = load_a(ab, 0, 0);
-#pragma unroll
-    for (int j = 0; j < FN; ++j) sw_[j] = load_scale(sb, in_period, 0, FM * WM + wn * FN + j);
-    s0 = load_scale(sb, in_period, 0, wm * FM);
-    a1 = load_a(ab, 0, 1);
-    s1 = load_scale(sb, in_period, 0, wm * FM + 1);
-  };
   bool stored = false;                             // the previous tile's STORES stores may still be on their way, issued after the loads
-  while (true) {
-#pragma unroll
-    for (int i = 0; i < FM; ++i)
-#pragma unroll
-      for (int j = 0; j < FN; ++j) acc[i][j] = f32x4_t{0, 0, 0, 0};
-    int v = v0;
-    bool last;
-    first_fragments(v0 & 3, wf[0], af[0], af[1], sw, sa[0], sa[1]);   // (not held over the results' way out)
-#pragma clang loop unroll(disable)
-    do {
-      auto products = [&](auto t_) {
-        constexpr int t = decltype(t_)::value, step = t / FM, i = t % FM;
-        __builtin_amdgcn_sched_barrier(0);
-        i32x8_t a = af[t % 3];
-        const int s = (int)sa[t % 3];
-        constexpr int OP = DIRECT ? 0 : step;
-        if constexpr (AF == A_E4M3_BANDS) {
-          const i32x8_t high = high_band(a);
-          a ^= high;
-#pragma unroll
-          for (int j = 0; j < FN; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[step][j], high, acc[i][j], 4, 0, OP, (int)(DIRECT && step ? sw1[j] : sw[j]), OP, s);
-        }
-#pragma unroll
-        for (int j = 0; j < FN; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[step][j], a, acc[i][j], 4, AF != A_E2M1 ? 0 : 4, OP, (int)(DIRECT && step ? sw1[j] : sw[j]), OP, s);
-        __builtin_amdgcn_sched_barrier(0);
-      };
-      for_each_int<0, N - 2>([&](auto t_) {
-        constexpr int t = decltype(t_)::value, step = t / FM, i = t % FM;
-        af[(t + 2) % 3] = load_a(ab, (t + 2) / FM, (t + 2) % FM);
-        sa[(t + 2) % 3] = load_scale(sb, v & 3, (t + 2) / FM, wm * FM + (t + 2) % FM);
-        if constexpr (step + 1 < T::STEPS) {
-#pragma unroll
-          for (int j = 0; j < FN; ++j)
-            if (FM - FN + j == i || (FM < FN && i == 0)) {
-              wf[1][j] = load_w(wb, 0, 1, j);
-              if constexpr (DIRECT) sw1[j] = load_scale(sb, 0, 1, FM * WM + wn * FN + j);
-            }
-        }
-        products(t_);
-      });
-#pragma unroll
-      for (int i = 0; i < FM; ++i)
-#pragma unroll
-        for (int j = 0; j < FN; ++j) asm volatile("" : "+v"(acc[i][j]));       // the products stay in front of the wait (no instruction)
-      // All of the stage is in registers.
-      wait_stage(stored);
-      stored = false;
-      last = v + T::STEPS >= steps;
-      const int next_v = last ? v0 : v + T::STEPS;
-      if (!DIRECT && f_period >= 0) turn_scales(f_period, sb ^ 1);
-      WAIT_LDS();
-      BARRIER();
-      ab = after(ab, NS);
-      if (AF == A_E2M1 || (next_v & 1) == 0 || last) wb = after(wb, NS);
-      if (DIRECT) sb = ab;
-      else if ((next_v & 3) == 0 || last) sb ^= 1;
-      i32x8_t w_next[FN], a0, a1;
-      uint32_t sw_next[FN], s0, s1;
-      first_fragments(next_v & 3, w_next, a0, a1, sw_next, s0, s1);
-      products(std::integral_constant<int, N - 2>{});
-#pragma unroll
-      for (int j = 0; j < FN; ++j) asm volatile("" : "+v"(acc[FM - 2][j]));    // (these stay in front of the asking)
-      fetch();
-      products(std::integral_constant<int, N - 1>{});
-#pragma unroll
-      for (int j = 0; j < FN; ++j) { wf[0][j] = w_next[j]; sw[j] = sw_next[j]; }
-      af[0] = a0; af[1] = a1; sa[0] = s0; sa[1] = s1;
-      v += T::STEPS;
-    } while (!last);
-
-    // Out, straight from the registers: of two neighbouring fragments a lane gets eight neighbouring columns of a row (16 bits), of one
-    // four (fp32); 16 rows x 64 bytes a store
+  // Out, straight from the registers: of two neighbouring fragments a lane gets eight neighbouring columns of a row (16 bits), of one
+  // four (fp32); 16 rows x 64 bytes a store
+  auto results = [&]() __attribute__((always_inline)) {
     int out_lane = lane;
     asm volatile("" : "+v"(out_lane));             // what follows from it is worked out here, not held in registers over the K loop
     const int row = m0 + wm * FM * 16 + (out_lane & 15), go = out_lane >> 4;
@@ -513,6 +424,220 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mx_gemm_kernel(const MxGemmPa
         __builtin_amdgcn_sched_barrier(0);
       }
     }
+  };
+
+  if constexpr (PAIRED) {
+    // The two rows of waves in turns: one reads a K step's fragments into registers and asks for rows to come, the other -- on the same
+    // SIMDs -- multiplies.  ROW 0 brings A, a K step ahead; ROW 1, half a step behind, brings W, a pair of steps ahead.  Step s is read in
+    // phase 2 s by ROW 0 and in phase 2 s + 1 by ROW 1, so its buffer is free from phase 2 s + 2 on, where ROW 0 asks for step s + 2; that
+    // has to be there by phase 2 s + 4, and ROW 0 waits for it behind its products of phase 2 s + 3.  W and, with the pairs of steps, its
+    // scales are waited for by ROW 1 where a pair is read for the last time.  A finished tile's results leave at the start of a phase,
+    // behind the asking, so that they may stay behind it (wait_stage).  Both rows pass 2 steps + 2 barriers.
+    auto turns = [&](auto row_) __attribute__((always_inline)) {
+      constexpr int ROW = decltype(row_)::value;
+      constexpr int ROWS = ROW == 0 ? BM : BN, PIECES = ROWS / 8 / WN, BUFFER = ROWS * 128;
+      const unsigned ld = ROW == 0 ? a_ld : w_ld;
+      unsigned off = (unsigned)((w % WN) * 8 + lr) * ld;
+      const unsigned to = __builtin_amdgcn_readfirstlane(lds0 + (unsigned)((ROW == 0 ? 0 : T::W_OFF) + (w % WN) * 1024));
+      auto ask_tile = [&]() __attribute__((always_inline)) {
+        tile_at(f_idx, f_m0, f_n0);
+        f_v = v0;
+        f_a = uniform(ROW == 0 ? p.a + (long)f_m0 * a_ld : p.w + ((long)f_n0 * w_ld - odd * 64));
+        f_sa = uniform(p.a_scale + ((long)f_m0 * s_ld - odd * 4));
+        f_sw = uniform(p.w_scale + ((long)f_n0 * s_ld - odd * 4));
+      };
+      auto ask = [&]() __attribute__((always_inline)) {
+        f_period = -1;
+        if (f_idx >= nwg) return;
+        const bool first = f_v == v0;
+        asm volatile("" : "+v"(off));                // its sums are worked out here, not held in registers
+        const unsigned plus = low + (ROW == 1 && first && odd ? lead : 0u);
+        const unsigned last = (unsigned)min(ROW == 0 ? p.M - 1 - f_m0 : p.N - 1 - f_n0, ROWS - 1) * ld;
+#pragma unroll
+        for (int i = 0; i < PIECES; ++i) dma16(f_a, min(off + (unsigned)(i * WN * 8) * ld, last) + plus, to + (unsigned)(f_ab * BUFFER + i * WN * 1024));
+        f_a += 128;
+        f_ab = after(f_ab, NS);
+        if ((f_v & 3) == 0 || first) {
+          f_period = f_v >> 2;
+          issue_scales(f_sa, f_sw, p.M - f_m0, p.N - f_n0, f_period);
+          f_sa += 16;
+          f_sw += 16;
+        }
+        if (ROW == 0 && first) {
+          if (p.bias) dma4((const uint8_t*)p.bias, (unsigned)min(f_n0 + tid, p.N - 1) * 4u, lds0 + (unsigned)(T::BIAS_OFF + f_bias * BN * 4 + w * 256));
+          f_bias = after(f_bias, T::NB);
+        }
+        f_v += ROW == 0 ? 1 : 2 - (f_v & 1);
+        if (f_v >= steps) {
+          f_idx += (int)gridDim.x;
+          if (f_idx < nwg) ask_tile();
+        }
+      };
+      auto wait = [&]() __attribute__((always_inline)) {
+        wait_stage(stored);
+        stored = false;
+        if (f_period >= 0) turn_scales(f_period, sb ^ 1);
+      };
+      ask_tile();
+      ask();
+      WAIT_ALL();
+      turn_scales(0, 0);
+      WAIT_LDS();
+      BARRIER();
+      if (ROW == 1) BARRIER();                       // half a step behind
+      bool asked = false;                            // in front of the results
+      i32x8_t wf[FN], af[FM];
+      uint32_t sa[FM], sw[FN];
+      while (true) {
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+          for (int j = 0; j < FN; ++j) acc[i][j] = f32x4_t{0, 0, 0, 0};
+        int v = v0;
+        bool last;
+#pragma clang loop unroll(disable)
+        do {
+          const bool opens = (v & 1) == 0 || v == v0, closes = (v & 1) != 0;       // its pair of steps
+#pragma unroll
+          for (int j = 0; j < FN; ++j) sw[j] = load_scale(sb, v & 3, 0, FM * WM + wn * FN + j);
+#pragma unroll
+          for (int i = 0; i < FM; ++i) sa[i] = load_scale(sb, v & 3, 0, wm * FM + i);
+#pragma unroll
+          for (int j = 0; j < FN; ++j) wf[j] = load_w(wb, v & 3, 0, j);
+#pragma unroll
+          for (int i = 0; i < FM; ++i) af[i] = load_a(ab, 0, i);
+          if (!asked && (ROW == 0 || opens)) ask();
+          asked = asked && ROW == 1 && !closes;
+          if (ROW == 1 && closes) wait();
+          WAIT_LDS();
+          BARRIER();
+#pragma unroll
+          for (int i = 0; i < FM; ++i) {
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+              acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[j], af[i], acc[i][j], 4, 0, 0, (int)sw[j], 0, (int)sa[i]);
+            __builtin_amdgcn_sched_barrier(0);
+          }
+#pragma unroll
+          for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) asm volatile("" : "+v"(acc[i][j]));   // the products stay in front of the wait (no instruction)
+          if (ROW == 0) wait();
+          WAIT_LDS();
+          BARRIER();
+          last = v + 1 >= steps;
+          ab = after(ab, NS);
+          if (closes) wb = after(wb, NS);
+          if ((v & 3) == 3 || last) sb ^= 1;
+          ++v;
+        } while (!last);
+        ask();
+        asked = true;
+        results();
+        bias_buf = after(bias_buf, T::NB);
+        idx += (int)gridDim.x;
+        if (idx >= nwg) break;
+        tile_at(idx, m0, n0);
+      }
+      if (ROW == 0) BARRIER();
+    };
+    if (wm == 0) turns(std::integral_constant<int, 0>{});
+    else turns(std::integral_constant<int, 1>{});
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < NS - 1; ++i) fetch();
+  wait_stage(false);
+  if (!DIRECT) turn_scales(0, 0);
+  WAIT_LDS();
+  BARRIER();
+  fetch();
+  i32x8_t wf[2][FN], af[3];
+  uint32_t sa[3], sw[FN], sw1[FN];               // sw1 (DIRECT): of the second step
+  auto first_fragments = [&](int in_period, i32x8_t (&w_)[FN], i32x8_t& a0, i32x8_t& a1, uint32_t (&sw_)[FN], uint32_t& s0, uint32_t& s1) {
+#pragma unroll
+    for (int j = 0; j < FN; ++j) w_[j] = load_w(wb, in_period, 0, j);
+    a0 = load_a(ab, 0, 0);
+#pragma unroll
+    for (int j = 0; j < FN; ++j) sw_[j] = load_scale(sb, in_period, 0, FM * WM + wn * FN + j);
+    s0 = load_scale(sb, in_period, 0, wm * FM);
+    a1 = load_a(ab, 0, 1);
+    s1 = load_scale(sb, in_period, 0, wm * FM + 1);
+  };
+  while (true) {
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j) acc[i][j] = f32x4_t{0, 0, 0, 0};
+    int v = v0;
+    bool last;
+    first_fragments(v0 & 3, wf[0], af[0], af[1], sw, sa[0], sa[1]);   // (not held over the results' way out)
+#pragma clang loop unroll(disable)
+    do {
+      auto products = [&](auto t_) {
+        constexpr int t = decltype(t_)::value, step = t / FM, i = t % FM;
+        __builtin_amdgcn_sched_barrier(0);
+        i32x8_t a = af[t % 3];
+        const int s = (int)sa[t % 3];
+        constexpr int OP = DIRECT ? 0 : step;
+        if constexpr (AF == A_E4M3_BANDS) {
+          const i32x8_t high = high_band(a);
+          a ^= high;
+#pragma unroll
+          for (int j = 0; j < FN; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[step][j], high, acc[i][j], 4, 0, OP, (int)(DIRECT && step ? sw1[j] : sw[j]), OP, s);
+        }
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[step][j], a, acc[i][j], 4, AF != A_E2M1 ? 0 : 4, OP, (int)(DIRECT && step ? sw1[j] : sw[j]), OP, s);
+        __builtin_amdgcn_sched_barrier(0);
+      };
+      for_each_int<0, N - 2>([&](auto t_) {
+        constexpr int t = decltype(t_)::value, step = t / FM, i = t % FM;
+        af[(t + 2) % 3] = load_a(ab, (t + 2) / FM, (t + 2) % FM);
+        sa[(t + 2) % 3] = load_scale(sb, v & 3, (t + 2) / FM, wm * FM + (t + 2) % FM);
+        if constexpr (step + 1 < T::STEPS) {
+#pragma unroll
+          for (int j = 0; j < FN; ++j)
+            if (FM - FN + j == i || (FM < FN && i == 0)) {
+              wf[1][j] = load_w(wb, 0, 1, j);
+              if constexpr (DIRECT) sw1[j] = load_scale(sb, 0, 1, FM * WM + wn * FN + j);
+            }
+        }
+        products(t_);
+      });
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j) asm volatile("" : "+v"(acc[i][j]));       // the products stay in front of the wait (no instruction)
+      // All of the stage is in registers.
+      wait_stage(stored);
+      stored = false;
+      last = v + T::STEPS >= steps;
+      const int next_v = last ? v0 : v + T::STEPS;
+      if (!DIRECT && f_period >= 0) turn_scales(f_period, sb ^ 1);
+      WAIT_LDS();
+      BARRIER();
+      ab = after(ab, NS);
+      if (AF == A_E2M1 || (next_v & 1) == 0 || last) wb = after(wb, NS);
+      if (DIRECT) sb = ab;
+      else if ((next_v & 3) == 0 || last) sb ^= 1;
+      i32x8_t w_next[FN], a0, a1;
+      uint32_t sw_next[FN], s0, s1;
+      first_fragments(next_v & 3, w_next, a0, a1, sw_next, s0, s1);
+      products(std::integral_constant<int, N - 2>{});
+#pragma unroll
+      for (int j = 0; j < FN; ++j) asm volatile("" : "+v"(acc[FM - 2][j]));    // (these stay in front of the asking)
+      fetch();
+      products(std::integral_constant<int, N - 1>{});
+#pragma unroll
+      for (int j = 0; j < FN; ++j) { wf[0][j] = w_next[j]; sw[j] = sw_next[j]; }
+      af[0] = a0; af[1] = a1; sa[0] = s0; sa[1] = s1;
+      v += T::STEPS;
+    } while (!last);
+
+    results();
     bias_buf = after(bias_buf, T::NB);
     idx += (int)gridDim.x;
     if (idx >= nwg) break;
@@ -704,16 +829,16 @@ hipError_t launch_few(const MxFewParams& p, hipStream_t stream) {
   return per >= 2 ? launch_few_u<T, AF, MF, 2>(p, stream) : launch_few_u<T, AF, MF, 1>(p, stream);
 }
 
-template <int AF, int BM, int BN, int WM, int WN, int NS, bool DIRECT>
+template <int AF, int BM, int BN, int WM, int WN, int NS, bool DIRECT, bool PAIRED = false>
 hipError_t launch(const MxGemmParams& p, hipStream_t stream) {
-  using T = Tile<AF, BM, BN, WM, WN, NS, DIRECT>;
+  using T = Tile<AF, BM, BN, WM, WN, NS, DIRECT, PAIRED>;
   static DeviceKernelSetup setup;
   int n_cu = 0;
-  if (hipError_t e = setup.ensure((const void*)mx_gemm_kernel<AF, BM, BN, WM, WN, NS, DIRECT>, T::LDS, &n_cu); e != hipSuccess) return e;
+  if (hipError_t e = setup.ensure((const void*)mx_gemm_kernel<AF, BM, BN, WM, WN, NS, DIRECT, PAIRED>, T::LDS, &n_cu); e != hipSuccess) return e;
   const long tiles = (long)((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN);
   if (tiles > 0x3fffffff) return hipErrorInvalidValue;
   const long resident = (long)n_cu * (163840 / T::LDS);             // workgroups that the CUs hold
-  hipLaunchKernelGGL((mx_gemm_kernel<AF, BM, BN, WM, WN, NS, DIRECT>), dim3((unsigned)(tiles < resident ? tiles : resident)), dim3(T::THREADS), T::LDS, stream, p);
+  hipLaunchKernelGGL((mx_gemm_kernel<AF, BM, BN, WM, WN, NS, DIRECT, PAIRED>), dim3((unsigned)(tiles < resident ? tiles : resident)), dim3(T::THREADS), T::LDS, stream, p);
   return hipGetLastError();
 }
 
@@ -730,31 +855,48 @@ hipError_t small_tiles(const MxGemmParams& p, hipStream_t stream) {
   else return launch<AF, 128, 128, 2, 4, 4, true>(p, stream);
 }
 
+// The few-row kernel: up to 64 rows, and more while its workgroups of 64 rows x 16 columns are at most one a CU -- a long K is then shared
+// by eight waves instead of walked by four: 256 x 4096 -> 1024, e2m1 / e4m3: 9.8 / 13.3 us, in 64 x 64 tiles 11.1 / 19.1; twice as many
+// workgroups: 384 rows 16.5 / 24.6 against 11.2 / 19.2.
+constexpr int CUS = 256;                // (a device with fewer CUs only takes its turns earlier)
+inline bool few(const MxGemmParams& p) { return p.M <= MX_FEW_ROWS || (long)((p.M + 63) / 64) * ((p.N + 15) / 16) <= CUS; }
+template <int AF>
+hipError_t few_rows(const MxGemmParams& p, hipStream_t stream) {
+  MxFewParams f{};
+  f.g = p;
+  return p.M <= 16 ? launch_few<void, AF, 1>(f, stream) : p.M <= 32 ? launch_few<void, AF, 2>(f, stream) : launch_few<void, AF, 4>(f, stream);
+}
+
+// 256 x 256 tiles.  e4m3 rows of 12 K steps on with the rows of waves in turns, which keeps the matrix pipe busier over a long K (4096 -> 1024,
+// 65 536 rows: 258 -> 221 us) but lets half the waves wait while the others' results leave (1024 -> 4096, 16 384 rows: 75.7 -> 80.1; 1280 -> 5120:
+// 146 -> 145).  e2m1 rows, whose products are half as long, lose by it (4096 -> 1024: 160 -> 178).
+template <int AF>
+hipError_t large_tiles(const MxGemmParams& p, hipStream_t stream) {
+  if constexpr (AF == A_E4M3)
+    if (p.nk >= 12) return launch<AF, 256, 256, 2, 4, 2, false, true>(p, stream);
+  return launch<AF, 256, 256, 2, 4, 2, false>(p, stream);
+}
+
 template <int AF>
 hipError_t choose(MxGemmParams p, hipStream_t stream) {
-  if (p.M <= MX_FEW_ROWS) {
-    MxFewParams f{};
-    f.g = p;
-    return p.M <= 16 ? launch_few<void, AF, 1>(f, stream) : p.M <= 32 ? launch_few<void, AF, 2>(f, stream) : launch_few<void, AF, 4>(f, stream);
-  }
-  // 256 x 256 tiles once they give every CU one (256 CUs; a device with fewer only gets them earlier).  Where a last round of them would
-  // leave three quarters of the CUs idle, its rows go to a second launch in small tiles: 65 792 x 4096 -> 1024 is 4 rounds and 4 tiles.
-  constexpr int CUS = 256;
+  if (few(p)) return few_rows<AF>(p, stream);
+  // 256 x 256 tiles once they give every CU one.  Where a last round of them would leave three quarters of the CUs idle, its rows go to a
+  // second launch of its own kind: 65 792 x 4096 -> 1024 is 4 rounds and 4 tiles.
   const long tn = (p.N + 255) / 256, tiles = (long)((p.M + 255) / 256) * tn;
   if (tiles < CUS) return small_tiles<AF>(p, stream);
   const int rest = (int)(tiles % CUS);
   const long rows = tiles / CUS * CUS / tn * 256;
-  if (rest == 0 || rest * 4 > CUS || rows == 0 || rows >= p.M) return launch<AF, 256, 256, 2, 4, 2, false>(p, stream);
+  if (rest == 0 || rest * 4 > CUS || rows == 0 || rows >= p.M) return large_tiles<AF>(p, stream);
   const int M = p.M;
   p.M = (int)rows;
-  if (hipError_t e = launch<AF, 256, 256, 2, 4, 2, false>(p, stream); e != hipSuccess) return e;
+  if (hipError_t e = large_tiles<AF>(p, stream); e != hipSuccess) return e;
   p.M = M - (int)rows;
   p.a += (size_t)rows * p.nk * (AF == A_E2M1 ? 64 : 128);
   p.a_scale += (size_t)rows * p.nk * 4;
   const size_t skip = (size_t)rows * p.N * (p.out_dtype == MX_DT_F32 ? 4 : 2);
   p.out = (char*)p.out + skip;
   if (p.resid) p.resid = (const char*)p.resid + skip;
-  return small_tiles<AF>(p, stream);
+  return few(p) ? few_rows<AF>(p, stream) : small_tiles<AF>(p, stream);
 }
 
 }  // namespace

@@ -290,6 +290,32 @@ def test_linear_of_more_tiles_than_the_gpu_holds(gpu, m, n, k, fmt):
 
 
 @pytest.mark.parametrize("fmt", ["e2m1", "e4m3"])
+@pytest.mark.parametrize("m,n,k", [(4097, 4104, 1500), (8300, 2048, 1601), (16640, 1024, 1537), (16700, 1100, 2000), (33100, 520, 1665), (130, 2000, 1700), (200, 1000, 2100), (256, 1024, 4096)])
+def test_linear_over_long_rows(gpu, m, n, k, fmt):
+    """One and more large tiles a workgroup over an even and an odd number of K steps, whole and ragged, a last round of few tiles; more rows
+    than 64 and few columns.  Bounds as in _check_linear."""
+    a, av = _random_coded(m, k, fmt, 3, gpu)
+    w, wv = _random_coded(n, k, "e2m1", 4, gpu)
+    a, av = mx.MXTensor(a.data, a.scale - 8, fmt, k), av * 2.0 ** -8
+    g = torch.Generator().manual_seed(k)
+    bias, res = (torch.randn(n, generator=g) * 100).to(gpu), (torch.randn(m, n, generator=g) * 100).to(torch.bfloat16).to(gpu)
+    aa, ww = torch.from_numpy(av).to(gpu), torch.from_numpy(wv).to(gpu)
+    size = aa.abs() @ ww.abs().t().contiguous() + bias.double().abs()
+    u = aa @ ww.t().contiguous() + bias.double()
+    cut = torch.from_numpy(np.asarray(_linear_cut(a, w, torch.bfloat16))).to(gpu)
+    pre = (128 + ora.padded(k) // 128 + 2) * U * size + cut
+
+    def check(y, want, tol):
+        assert ((y.double() - want).abs() <= tol + 2 * U * want.abs() + 2.0 ** -8 * (want.abs() + tol)).all()
+
+    for _ in range(2):
+        check(mx.linear(a, w, bias=bias, residual=res), u + res.double(), pre)
+        check(mx.linear(a, w), u - bias.double(), pre)
+        want = u * 0.5 * (1 + torch.erf(u / 2 ** 0.5))
+        check(mx.linear(a, w, bias=bias, act="gelu"), want, 1.13 * pre + 16 * U * want.abs() + 1.5e-7 * u.abs())
+
+
+@pytest.mark.parametrize("fmt", ["e2m1", "e4m3"])
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("m,n,k", [(1, 1664, 1280), (1, 33, 77), (7, 500, 300), (16, 256, 2048), (17, 128, 640), (40, 200, 4096), (64, 320, 1001), (65, 96, 512), (300, 130, 200)])
 def test_linear_of_values_is_quantize_and_linear(gpu, m, n, k, dtype, fmt):
