@@ -105,7 +105,7 @@ SIGNATURES = {
                                          c_void_p, c_void_p, c_void_p, c_void_p]),
     "clipenc_op_gemm_mx": (c_int, [c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p,
                                    c_int, c_void_p]),
-    "clipenc_op_linear_mx_ws_bytes": (c_size_t, [c_int, c_int, c_int]),
+    "clipenc_op_linear_mx_ws_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
     "clipenc_op_linear_mx": (c_int, [c_void_p, c_int, c_long, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_int, c_void_p,
                                      c_void_p, c_int, c_void_p, c_size_t, c_void_p]),
     "clipenc_forward_tokens": (c_int, [c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p]),

@@ -1459,8 +1459,8 @@ int clipenc_op_gemm_mx(const void* a_dev, const void* a_scale_dev, int a_fmt, co
   return 0;
 }
 
-size_t clipenc_op_linear_mx_ws_bytes(int m, int k, int x_fmt) {
-  if (m <= MX_VALUE_ROWS || k < 1 || k > MX_MAX_K || (x_fmt != CLIPENC_MX_E2M1 && x_fmt != CLIPENC_MX_E4M3)) return 0;
+size_t clipenc_op_linear_mx_ws_bytes(int m, int n, int k, int x_fmt) {
+  if (m < 1 || n < 1 || mx_takes_values(m, n, k) || k < 1 || k > MX_MAX_K || (x_fmt != CLIPENC_MX_E2M1 && x_fmt != CLIPENC_MX_E4M3)) return 0;
   return (size_t)m * (mx_row_bytes(k, x_fmt) + (size_t)mx_kp(k) / 32);
 }
 
@@ -1471,9 +1471,9 @@ int clipenc_op_linear_mx(const void* in_dev, int in_dtype, long ld_in, int x_fmt
   if (int rc = mx_check_rows("linear_mx", in_dev, in_dtype, m, k, ld_in)) return rc;
   if (x_fmt != CLIPENC_MX_E2M1 && x_fmt != CLIPENC_MX_E4M3) return fail("linear_mx: x_fmt = %d (CLIPENC_MX_E2M1 or CLIPENC_MX_E4M3)", x_fmt);
   if (m == 0 || n == 0) return 0;
-  const size_t need = clipenc_op_linear_mx_ws_bytes(m, k, x_fmt);
+  const size_t need = clipenc_op_linear_mx_ws_bytes(m, n, k, x_fmt);
   if (need && (!ws_dev || ws_bytes < need || !aligned_to(ws_dev, 16))) return fail("linear_mx: scratch of %zu bytes, 16-byte aligned, is needed: %zu given", need, ws_dev ? ws_bytes : (size_t)0);
-  if (m <= MX_VALUE_ROWS) {
+  if (mx_takes_values(m, n, k)) {
     MxGemmParams p{};
     p.w = (const uint8_t*)w_dev; p.w_scale = (const uint8_t*)w_scale_dev; p.M = m; p.N = n; p.nk = mx_kp(k) / 128; p.bias = bias_dev;
     p.resid = resid_dev; p.out = out_dev; p.act = act; p.out_dtype = out_dtype;

@@ -646,10 +646,13 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mx_gemm_kernel(const MxGemmPa
 }
 
 // ---- few rows -----------------------------------------------------------------------------------------------------------------------
-// Up to 64 rows: 16 columns n a workgroup, whose waves share K and add their sums up in LDS, in wave order.  Fragments come straight from
+// Few rows, or few columns: 16 columns n a workgroup, whose waves share K and add their sums up in LDS, in wave order.  Fragments come straight from
 // memory -- each byte of W is read once, and there is nothing to wait for but that one read: a tile walk of the same product pays a
 // memory latency a stage.  SRC: quantised rows (MX_E2M1 / MX_E4M3), or values of type T that the lanes quantise themselves, with the
-// codes of clipenc_op_quant_mx (up to 16 rows: each workgroup does it again).
+// codes of clipenc_op_quant_mx; each workgroup does it again, so beyond MX_VALUE_COLS columns it has 64 of them (12 800 x 5120, one row:
+// 15 us instead of 24; 4096 x 1024, whose workgroups are then a quarter of the CUs: 6.3 instead of 4.5).
+// One row of 8192 x 1664 takes 4.2 us from codes, whose 7 MB of weights are 1.4 us of HBM and whose launch and one trip to memory are the
+// rest; 12 800 x 5120 (33 MB) 11.7 us, 2.9 TB/s.
 struct MxFewParams {
   MxGemmParams g;
   const void* x; long ld_x; int k;                // values: [M] rows of k
@@ -717,7 +720,7 @@ __device__ __forceinline__ void load16(const T* row, int c, int k, float* v) {
   }
 }
 
-constexpr int FEW_WAVES = 8;
+constexpr int FEW_WAVES = 8, MX_VALUE_COLS = 8192;
 
 // Scale words of U neighbouring K steps of a row, the lane's byte lowest
 template <int U>
@@ -728,36 +731,43 @@ __device__ __forceinline__ void load_words(const uint8_t* scales, size_t step, i
   for (int u = 0; u < U; ++u) s[u] = w.v[u] >> (8 * g);
 }
 
-// T = void: the rows are quantised;  AF: A_*;  MF: 16-row fragments;  U: K steps whose loads are under way together.  A wave has
+// T = void: the rows are quantised;  AF: A_*;  MF, NF: 16-row and 16-column fragments;  U: K steps whose loads are under way together.  A wave has
 // neighbouring steps, so that it reads whole lines of its rows and the scales of U steps at once.
-template <typename T, int AF, int MF, int U>
+template <typename T, int AF, int MF, int NF, int U>
 __global__ __launch_bounds__(FEW_WAVES * 64) void mx_few_kernel(const MxFewParams fp) {
   const MxGemmParams& p = fp.g;
   constexpr bool VALUES = !std::is_same<T, void>::value;
   constexpr int FMT = AF == A_E2M1 ? MX_E2M1 : MX_E4M3;
-  __shared__ __attribute__((aligned(16))) float sums[FEW_WAVES][MF][256];
+  __shared__ __attribute__((aligned(16))) float sums[FEW_WAVES][MF * NF][256];
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6), waves = blockDim.x >> 6;
-  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * (MF * 16);
-  const size_t w_row = (size_t)min(n0 + r16, p.N - 1) * p.nk;                      // in K steps
-  size_t a_row[MF];
+  const int n0 = blockIdx.x * (NF * 16), m0 = blockIdx.y * (MF * 16);
+  size_t w_row[NF], a_row[MF];                                                     // in K steps
+#pragma unroll
+  for (int j = 0; j < NF; ++j) w_row[j] = (size_t)min(n0 + j * 16 + r16, p.N - 1) * p.nk;
 #pragma unroll
   for (int i = 0; i < MF; ++i) a_row[i] = (size_t)min(m0 + i * 16 + r16, p.M - 1) * (VALUES ? (size_t)fp.ld_x : (size_t)p.nk);
-  f32x4_t acc[MF];
+  f32x4_t acc[MF][NF];
 #pragma unroll
-  for (int i = 0; i < MF; ++i) acc[i] = f32x4_t{0, 0, 0, 0};
+  for (int i = 0; i < MF; ++i)
+#pragma unroll
+    for (int j = 0; j < NF; ++j) acc[i][j] = f32x4_t{0, 0, 0, 0};
   auto steps = [&](int ks, auto n_) {
     constexpr int C = decltype(n_)::value;
-    i32x8_t wf[C], af[C][MF];
-    uint32_t sw[C], sa[MF][C];
-    load_words<C>(p.w_scale, w_row + ks, g, sw);
+    i32x8_t wf[C][NF], af[C][MF];
+    uint32_t sw[NF][C], sa[MF][C];
+#pragma unroll
+    for (int j = 0; j < NF; ++j) load_words<C>(p.w_scale, w_row[j] + ks, g, sw[j]);
 #pragma unroll
     for (int i = 0; i < MF; ++i)
       if constexpr (!VALUES) load_words<C>(p.a_scale, a_row[i] + ks, g, sa[i]);
 #pragma unroll
     for (int u = 0; u < C; ++u) {
-      const i32x4_t v = *(const i32x4_t*)(p.w + (w_row + ks + u) * 64 + g * 16);
-      wf[u] = __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1);
+#pragma unroll
+      for (int j = 0; j < NF; ++j) {
+        const i32x4_t v = *(const i32x4_t*)(p.w + (w_row[j] + ks + u) * 64 + g * 16);
+        wf[u][j] = __builtin_shufflevector(v, v, 0, 1, 2, 3, -1, -1, -1, -1);
+      }
 #pragma unroll
       for (int i = 0; i < MF; ++i) {
         if constexpr (VALUES) {
@@ -786,9 +796,13 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void mx_few_kernel(const MxFewParam
         if constexpr (AF == A_E4M3_BANDS) {
           const i32x8_t high = high_band(a);
           a ^= high;
-          acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[u], high, acc[i], 4, 0, 0, (int)sw[u], 0, (int)sa[i][u]);
+#pragma unroll
+          for (int j = 0; j < NF; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[u][j], high, acc[i][j], 4, 0, 0, (int)sw[j][u], 0, (int)sa[i][u]);
         }
-        acc[i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[u], a, acc[i], 4, AF != A_E2M1 ? 0 : 4, 0, (int)sw[u], 0, (int)sa[i][u]);
+#pragma unroll
+        for (int j = 0; j < NF; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[u][j], a, acc[i][j], 4, AF != A_E2M1 ? 0 : 4, 0, (int)sw[j][u], 0, (int)sa[i][u]);
       }
   };
   const int per = (p.nk + waves - 1) / waves, end = min((w + 1) * per, p.nk);
@@ -797,10 +811,12 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void mx_few_kernel(const MxFewParam
   if constexpr (U > 1)
     for (; ks < end; ++ks) steps(ks, std::integral_constant<int, 1>{});
 #pragma unroll
-  for (int i = 0; i < MF; ++i) *(f32x4_t*)&sums[w][i][r16 * 16 + g * 4] = acc[i];   // row r16, columns 4 g .. 4 g + 3
+  for (int i = 0; i < MF; ++i)
+#pragma unroll
+    for (int j = 0; j < NF; ++j) *(f32x4_t*)&sums[w][i * NF + j][r16 * 16 + g * 4] = acc[i][j];   // row r16, columns 4 g .. 4 g + 3
   __syncthreads();
-  for (int t = tid; t < MF * 256; t += blockDim.x) {
-    const int m = m0 + t / 16, n = n0 + (t & 15);
+  for (int t = tid; t < MF * NF * 256; t += blockDim.x) {
+    const int m = m0 + t / (NF * 256) * 16 + (t & 255) / 16, n = n0 + t / 256 % NF * 16 + (t & 15);
     float v = 0.0f;
     for (int i = 0; i < waves; ++i) v += sums[i][t / 256][t & 255];
     if (m < p.M && n < p.N) {
@@ -813,20 +829,20 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void mx_few_kernel(const MxFewParam
   }
 }
 
-template <typename T, int AF, int MF, int U>
+template <typename T, int AF, int MF, int NF, int U>
 hipError_t launch_few_u(const MxFewParams& p, hipStream_t stream) {
   const int waves = p.g.nk < FEW_WAVES ? p.g.nk : FEW_WAVES;
-  hipLaunchKernelGGL((mx_few_kernel<T, AF, MF, U>), dim3((unsigned)((p.g.N + 15) / 16), (unsigned)((p.g.M + MF * 16 - 1) / (MF * 16))), dim3((unsigned)waves * 64), 0,
-                     stream, p);
+  const dim3 grid((unsigned)((p.g.N + NF * 16 - 1) / (NF * 16)), (unsigned)((p.g.M + MF * 16 - 1) / (MF * 16)));
+  hipLaunchKernelGGL((mx_few_kernel<T, AF, MF, NF, U>), grid, dim3((unsigned)waves * 64), 0, stream, p);
   return hipGetLastError();
 }
 // as many steps under way as a wave has, and its registers hold
-template <typename T, int AF, int MF>
+template <typename T, int AF, int MF, int NF = 1>
 hipError_t launch_few(const MxFewParams& p, hipStream_t stream) {
   const int per = (p.g.nk + FEW_WAVES - 1) / FEW_WAVES;
   if constexpr (std::is_same<T, void>::value && MF <= 2)
-    if (per >= 4) return launch_few_u<T, AF, MF, 4>(p, stream);
-  return per >= 2 ? launch_few_u<T, AF, MF, 2>(p, stream) : launch_few_u<T, AF, MF, 1>(p, stream);
+    if (per >= 4) return launch_few_u<T, AF, MF, NF, 4>(p, stream);
+  return per >= 2 ? launch_few_u<T, AF, MF, NF, 2>(p, stream) : launch_few_u<T, AF, MF, NF, 1>(p, stream);
 }
 
 template <int AF, int BM, int BN, int WM, int WN, int NS, bool DIRECT, bool PAIRED = false>
@@ -855,11 +871,12 @@ hipError_t small_tiles(const MxGemmParams& p, hipStream_t stream) {
   else return launch<AF, 128, 128, 2, 4, 4, true>(p, stream);
 }
 
-// The few-row kernel: up to 64 rows, and more while its workgroups of 64 rows x 16 columns are at most one a CU -- a long K is then shared
-// by eight waves instead of walked by four: 256 x 4096 -> 1024, e2m1 / e4m3: 9.8 / 13.3 us, in 64 x 64 tiles 11.1 / 19.1; twice as many
-// workgroups: 384 rows 16.5 / 24.6 against 11.2 / 19.2.
+// The few-row kernel: up to 16 rows; up to 48 while its workgroups are at most two a CU (e2m1 / e4m3, 48 rows: 8192 columns of 1664
+// 5.9 / 10.1 us, in 64 x 64 tiles 8.5 / 11.9; 12 800 columns of 5120 28 / 47 against 16 / 27); more rows while its workgroups of 64 rows x
+// 16 columns are at most one a CU -- a long K is then shared by eight waves instead of walked by four (256 x 4096 -> 1024 9.8 / 13.3 us
+// against 11.1 / 19.1; 384 rows 16.5 / 24.6 against 11.2 / 19.2).
 constexpr int CUS = 256;                // (a device with fewer CUs only takes its turns earlier)
-inline bool few(const MxGemmParams& p) { return p.M <= MX_FEW_ROWS || (long)((p.M + 63) / 64) * ((p.N + 15) / 16) <= CUS; }
+inline bool few(const MxGemmParams& p) { return p.M <= 16 || (long)((p.M + 63) / 64) * ((p.N + 15) / 16) <= (p.M <= 48 ? 2 * CUS : CUS); }
 template <int AF>
 hipError_t few_rows(const MxGemmParams& p, hipStream_t stream) {
   MxFewParams f{};
@@ -909,13 +926,17 @@ hipError_t ce_mx_gemm(MxGemmParams p, int a_fmt, hipStream_t stream) {
   return p.out_dtype == MX_DT_F32 ? choose<A_E4M3_BANDS>(p, stream) : choose<A_E4M3>(p, stream);
 }
 
+template <typename T, int AF>
+static hipError_t few_values_of(const MxFewParams& f, hipStream_t stream) {
+  return f.g.N > MX_VALUE_COLS ? launch_few<T, AF, 1, 4>(f, stream) : launch_few<T, AF, 1>(f, stream);
+}
 template <typename T>
 static hipError_t few_values(const MxFewParams& f, int fmt, hipStream_t stream) {
-  if (fmt == MX_E2M1) return launch_few<T, A_E2M1, 1>(f, stream);
-  return f.g.out_dtype == MX_DT_F32 ? launch_few<T, A_E4M3_BANDS, 1>(f, stream) : launch_few<T, A_E4M3, 1>(f, stream);
+  if (fmt == MX_E2M1) return few_values_of<T, A_E2M1>(f, stream);
+  return f.g.out_dtype == MX_DT_F32 ? few_values_of<T, A_E4M3_BANDS>(f, stream) : few_values_of<T, A_E4M3>(f, stream);
 }
 hipError_t ce_mx_gemm_values(const MxGemmParams& p, const void* x, int dtype, long ld_x, int k, int fmt, hipStream_t stream) {
-  if (p.M > MX_VALUE_ROWS) return hipErrorInvalidValue;
+  if (!mx_takes_values(p.M, p.N, k)) return hipErrorInvalidValue;
   MxFewParams f{};
   f.g = p; f.x = x; f.ld_x = ld_x; f.k = k;
   return dtype == MX_DT_BF16 ? few_values<__bf16>(f, fmt, stream) : dtype == MX_DT_F16 ? few_values<_Float16>(f, fmt, stream) : few_values<float>(f, fmt, stream);

@@ -13,10 +13,14 @@ enum { MX_DT_BF16 = 0, MX_DT_F16 = 1, MX_DT_F32 = 2 };
 enum { MX_NORM_RMS = 0, MX_NORM_LAYER = 1 };
 #define MX_NORM_MAX_K 16384             // widest row of the norm: 1024 threads hold it in registers, 16 values each
 
-#define MX_FEW_ROWS 64                  // products of so few rows read their fragments straight from memory
-#define MX_VALUE_ROWS 16                // products of so few rows take values and quantise them themselves
-
 static inline int mx_kp(int k) { return (k + 127) / 128 * 128; }
+// Whether a product quantises its rows itself, one launch instead of two, in every workgroup again: up to 16 rows, and up to 64 while the
+// workgroups of 16 x 16 results are two a CU or fewer (4096 x 1024, e4m3, GPU time of 1 / 32 rows: 4.5 / 6.4 us, in two launches 5.6 / 7.3;
+// 5120 x 1280, 24 rows: 9.9 against 8.1) -- and no more than 2^26 weights, whose sweep would be held up by it (12 800 x 5120, 1 / 16 rows:
+// 15 / 16 us against 14 / 21; 8192 x 8192: 20 / 24 against 12 / 18).
+static inline bool mx_takes_values(int m, int n, int k) {
+  return (m <= 16 || (m <= 64 && (long)((m + 15) / 16) * ((n + 15) / 16) <= 512)) && (long)n * k < 1l << 26;
+}
 
 struct MxNormParams {
   const void* x; long ld_x;             // [n_rows] rows of k elements, ld_x elements apart
@@ -78,5 +82,5 @@ hipError_t ce_mx_quant(const void* x, int dtype, long n_rows, int k, long ld_x, 
 hipError_t ce_mx_dequant(const uint8_t* q, const void* scale, int fmt, long n_rows, int k, void* out, int out_dtype, hipStream_t stream);
 hipError_t ce_mx_norm(const MxNormParams& p, int dtype, hipStream_t stream);
 hipError_t ce_mx_gemm(MxGemmParams p, int a_fmt, hipStream_t stream);
-// p.M <= MX_VALUE_ROWS: the rows of p.a are quantised from x inside
+// mx_takes_values: the rows of p.a are quantised from x inside
 hipError_t ce_mx_gemm_values(const MxGemmParams& p, const void* x, int dtype, long ld_x, int k, int fmt, hipStream_t stream);

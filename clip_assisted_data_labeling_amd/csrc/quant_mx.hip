@@ -16,7 +16,10 @@
 
 namespace {
 
-constexpr int QUANT_ROWS = 1, QUANT_BLOCKS = 256 * 256, DEQUANT_ROWS = 4, DEQUANT_BLOCKS = 256 * 8;
+// 65 792 x 4096 of bf16 to e2m1 and back, 682 MB each: 117 us (5.8 TB/s) and 137 us (5.0).  Quantising wants many short workgroups -- one row
+// a thread and step: 256 workgroups a CU 117 us, 64 131; four rows in flight and 16 a CU 154 --, reading back few long ones: four rows in
+// flight and 8 a CU 137 us, 16 a CU 145, one row 182.
+constexpr int QUANT_BLOCKS = 256 * 256, DEQUANT_ROWS = 4, DEQUANT_BLOCKS = 256 * 8;
 
 typedef __attribute__((ext_vector_type(4))) uint32_t u32x4_t;
 typedef mx_u32x2_t u32x2_t;
@@ -124,7 +127,7 @@ __device__ __forceinline__ void store_block(const float (&v)[8], int fmt, uint8_
 }
 
 // Threads 0 .. active - 1 own (row, 8 columns) pairs, row by row; active is a multiple of kp / 8, so that a step of the loop moves
-// every thread by `step` = active / (kp / 8) whole rows.  Four rows a thread are in flight.
+// every thread by `step` = active / (kp / 8) whole rows.
 template <typename T, int FMT, bool WHOLE>
 __global__ __launch_bounds__(256) void mx_quant_kernel(const T* __restrict__ x, long n_rows, int k, int kp, long ld_x, uint8_t* __restrict__ q,
                                                        uint8_t* __restrict__ scale, long active, long step) {
@@ -134,20 +137,7 @@ __global__ __launch_bounds__(256) void mx_quant_kernel(const T* __restrict__ x, 
   const long row0 = id / per_row;
   const int c = (int)(id - row0 * per_row) * 8;
   const size_t q_ld = FMT == MX_E2M1 ? kp / 2 : kp, s_ld = kp / 32;
-  constexpr int R = QUANT_ROWS;
-  long row = row0;
-  for (; row + (R - 1) * step < n_rows; row += R * step) {
-    Raw<T> r[R];
-#pragma unroll
-    for (int i = 0; i < R; ++i) r[i] = load_raw<T, WHOLE>(x + (row + i * step) * ld_x, c, k);
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      float v[8];
-      values_of(r[i], v);
-      store_block(v, FMT, q + (size_t)(row + i * step) * q_ld, scale + (size_t)(row + i * step) * s_ld, c);
-    }
-  }
-  for (; row < n_rows; row += step) {
+  for (long row = row0; row < n_rows; row += step) {
     float v[8];
     values_of(load_raw<T, WHOLE>(x + row * ld_x, c, k), v);
     store_block(v, FMT, q + (size_t)row * q_ld, scale + (size_t)row * s_ld, c);
@@ -158,7 +148,7 @@ __device__ __forceinline__ float scale_value(uint32_t x) {
   return x == 0xffu ? __builtin_nanf("") : x ? __uint_as_float(x << 23) : 0x1p-127f;
 }
 
-// (row, 8 columns) pairs as above; the elements and scales of four rows are in flight
+// (row, 8 columns) pairs as above; the elements and scales of DEQUANT_ROWS rows are in flight
 template <typename T, int FMT, bool WHOLE>
 __global__ __launch_bounds__(256) void mx_dequant_kernel(const uint8_t* __restrict__ q, const void* __restrict__ scale, long n_rows, int k, int kp,
                                                          T* __restrict__ out, long active, long step) {
@@ -219,17 +209,9 @@ __global__ __launch_bounds__(256) void mx_dequant_kernel(const uint8_t* __restri
 //   h = x + resid (rounded to the rows' type, as it is stored);  RMS: y = h / sqrt(mean(h^2) + eps) * gamma + beta,
 //   LAYER: the same of h - mean(h);  then y in blocks, or in e4m3 with one scale a row, max|y| / 448
 // The row stays in the registers of NT threads, CH chunks of 8 columns each, and so does its share of gamma; the next row's loads are
-// under way while a row is worked on.  Sums, the factor and y are formed in 64 bits -- fp64 runs at the rate of unpacked fp32
-// here and hides behind the row's bytes -- and y reaches its few bits through an fp32 value rounded to ODD, so that codes are those
-// of the 64-bit y: no square overflows, and no value next to a rounding border is rounded twice.
-__device__ __forceinline__ float to_odd(double d) {
-  const float f = (float)d;
-  const double left = d - (double)f;
-  uint32_t b = __float_as_uint(f);
-  if (left != 0.0) b = (b - (((left < 0.0) != (f < 0.0)) ? 1u : 0u)) | 1u;      // |f| > |d|: one step back; inexact: odd
-  return __uint_as_float(b);                                                    // (inf and NaN stay not finite)
-}
-
+// under way while a row is worked on.  Sums, the factor and y are formed in 64 bits, so that no square overflows and beta may cancel; y
+// is rounded to fp32 and from there to its few bits: a value within 2^-24 of a border between two codes may take either.
+// 65 536 rows of 1024, bf16, with residual and h: 470 MB in 92 us (5.1 TB/s, what a copy reaches); of 1280 without: 254 MB in 68 us.
 template <int NT>
 __device__ __forceinline__ double sum_over(double v, double* red) {
 #pragma unroll
@@ -298,7 +280,8 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void mx_norm_kernel(const MxNo
     }
     if (row + per_step < p.n_rows) fetch(row + per_step);
     double mean = 0;
-    if (p.norm == MX_NORM_LAYER) {
+    const bool layer = p.norm == MX_NORM_LAYER;
+    if (layer) {
       double s = 0;
 #pragma unroll
       for (int i = 0; i < CH; ++i)
@@ -307,22 +290,39 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void mx_norm_kernel(const MxNo
       mean = sum_over<NT>(s, red) / p.k;
     }
     double ss = 0;
+    if (layer) {
 #pragma unroll
-    for (int i = 0; i < CH; ++i)
+      for (int i = 0; i < CH; ++i)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const double d = inside(i, j) ? (double)v[i][j] - mean : 0.0;
-        ss = fma(d, d, ss);
-      }
+        for (int j = 0; j < 8; ++j) {
+          const double d = inside(i, j) ? (double)v[i][j] - mean : 0.0;
+          ss = fma(d, d, ss);
+        }
+    } else {
+#pragma unroll
+      for (int i = 0; i < CH; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ss = fma((double)v[i][j], (double)v[i][j], ss);   // (behind the row: zeros)
+    }
     const double factor = 1.0 / sqrt(sum_over<NT>(ss, red) / p.k + (double)p.eps);
     auto y_of = [&](int i, double (&y)[8]) {
-      float b[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-      if (p.beta) values_of(load_raw<float, WHOLE>(p.beta, (i * NT + t) * 8, p.k), b);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      auto of = [&](int j) {
         float gj = g[i][j];
         asm("" : "+v"(gj));                                                     // kept as fp32: its conversion is not to leave the loop
-        y[j] = inside(i, j) ? fma(((double)v[i][j] - mean) * factor, (double)gj, (double)b[j]) : 0.0;
+        return (double)gj * factor;
+      };
+      if (layer) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = inside(i, j) ? ((double)v[i][j] - mean) * of(j) : 0.0;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = (double)v[i][j] * of(j);
+      }
+      if (p.beta) {
+        float b[8];
+        values_of(load_raw<float, WHOLE>(p.beta, (i * NT + t) * 8, p.k), b);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] += (double)b[j];
       }
     };
     if constexpr (ROW) {
@@ -346,7 +346,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void mx_norm_kernel(const MxNo
         y_of(i, y);
         float f[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = to_odd(y[j] * inv);
+        for (int j = 0; j < 8; ++j) f[j] = (float)(y[j] * inv);
         u32x2_t w = mx_to_e4m3(f, 1.0f);
         if (!fine) w = u32x2_t{0u, 0u};
         if (c < p.kp) *(u32x2_t*)(p.q + (size_t)row * p.kp + c) = w;
@@ -360,7 +360,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void mx_norm_kernel(const MxNo
         y_of(i, y);
         float f[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = to_odd(y[j]);
+        for (int j = 0; j < 8; ++j) f[j] = (float)y[j];
         if (c < p.kp) store_block(f, p.fmt, p.q + (size_t)row * q_ld, (uint8_t*)p.scale + (size_t)row * (p.kp / 32), c);
       }
     }
@@ -400,6 +400,11 @@ void launch_dequant(const uint8_t* q, const void* scale, int fmt, long n_rows, i
 #undef DEQUANT_LAUNCH
 }
 
+// Threads of a row: as few as hold it in 24 .. 32 values each, since every wave more costs a turn of the sums (65 536 rows of 1280 / 2048 / 4096 /
+// 8192, bf16 to e4m3: 68 / 105 / 194 / 354 us; in 256 / 256 / 512 / 1024 threads of 8 values 104 / 118 / 276 / 605; 512 columns as 64 x 8 35
+// us, as 256 x 8 97).  Up to NORM_FEW rows of up to 2048 the latency of one row counts: 256 threads of 8 values (one row of 1280 3.8 us instead
+// of 4.4, 1024 rows 5.3 both, 2048 rows 7.3 instead of 6.1).
+constexpr long NORM_FEW = 1024;
 template <typename T, bool WHOLE>
 hipError_t launch_norm(const MxNormParams& p, hipStream_t stream) {
   const long waves = (p.n_rows + 3) / 4;
@@ -409,10 +414,12 @@ hipError_t launch_norm(const MxNormParams& p, hipStream_t stream) {
   else hipLaunchKernelGGL((mx_norm_kernel<T, NT, CH, WHOLE, false>), dim3(NT == 64 ? g4 : g1), dim3(NT == 64 ? 256 : NT), 0, stream, p)
   if (p.kp <= 512) { NORM_LAUNCH(64, 1); }
   else if (p.kp <= 1024) { NORM_LAUNCH(64, 2); }
-  else if (p.kp <= 2048) { NORM_LAUNCH(256, 1); }
-  else if (p.kp <= 4096) { NORM_LAUNCH(512, 1); }
-  else if (p.kp <= 8192) { NORM_LAUNCH(1024, 1); }
-  else if (p.kp <= MX_NORM_MAX_K) { NORM_LAUNCH(1024, 2); }
+  else if (p.kp <= 2048 && p.n_rows <= NORM_FEW) { NORM_LAUNCH(256, 1); }
+  else if (p.kp <= 1536) { NORM_LAUNCH(64, 3); }
+  else if (p.kp <= 2048) { NORM_LAUNCH(128, 2); }
+  else if (p.kp <= 4096) { NORM_LAUNCH(256, 2); }
+  else if (p.kp <= 8192) { NORM_LAUNCH(256, 4); }
+  else if (p.kp <= MX_NORM_MAX_K) { NORM_LAUNCH(512, 4); }
   else return hipErrorInvalidValue;
 #undef NORM_LAUNCH
   return hipGetLastError();

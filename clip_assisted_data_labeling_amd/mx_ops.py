@@ -215,7 +215,7 @@ def linear(x, w: MXTensor, bias: Optional[torch.Tensor] = None, act: Optional[st
               out.data_ptr(), out_dt)
         return out
     ws = None
-    need = lib.clipenc_op_linear_mx_ws_bytes(rows, cols, fmt)
+    need = lib.clipenc_op_linear_mx_ws_bytes(rows, n, cols, fmt)
     if need:
         scratch = _empty((need,), (1,), dtype=torch.uint8, device=device)
         ws = scratch.data_ptr()

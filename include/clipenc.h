@@ -374,7 +374,8 @@ int clipenc_op_dequant_mx(const void* q_dev, const void* scale_dev, int fmt, lon
  *   y = h * gamma / sqrt(mean(h^2) + eps) + beta             norm = CLIPENC_NORM_RMS
  *       (h - mean(h)) * gamma / sqrt(var(h) + eps) + beta           CLIPENC_NORM_LAYER       (beta_dev may be NULL)
  * and y in fmt (any of the three).  gamma / beta: float [k]; k <= 16384; ld_in / ld_resid in elements; h_out_dev may be in_dev or
- * resid_dev where that one's rows are k elements apart.  Sums and the row's factor are held in 64 bits. */
+ * resid_dev where that one's rows are k elements apart.  Sums, the row's factor and y are formed
+ * in 64 bits; y is rounded to fp32 once, then to its few. */
 int clipenc_op_norm_quant_mx(const void* in_dev, int in_dtype, long n_rows, int k, long ld_in, const void* resid_dev, long ld_resid, int norm,
                              const float* gamma_dev, const float* beta_dev, float eps, int fmt, void* h_out_dev, void* out_dev,
                              void* scale_dev, void* stream);
@@ -384,8 +385,8 @@ int clipenc_op_norm_quant_mx(const void* in_dev, int in_dtype, long n_rows, int 
 int clipenc_op_gemm_mx(const void* a_dev, const void* a_scale_dev, int a_fmt, const void* w_dev, const void* w_scale_dev, int m, int n, int k,
                        const float* bias_dev, int act, const void* resid_dev, void* out_dev, int out_dtype, void* stream);
 /* The same from values: A = quantised `in` (as clipenc_op_quant_mx to x_fmt), in one call.  ws_dev: 16-byte aligned scratch of
- * clipenc_op_linear_mx_ws_bytes(m, k, x_fmt) bytes (0 where the product takes the values as they are: ws_dev may be NULL then). */
-size_t clipenc_op_linear_mx_ws_bytes(int m, int k, int x_fmt);
+ * clipenc_op_linear_mx_ws_bytes(m, n, k, x_fmt) bytes (0 where the product takes the values as they are: ws_dev may be NULL then). */
+size_t clipenc_op_linear_mx_ws_bytes(int m, int n, int k, int x_fmt);
 int clipenc_op_linear_mx(const void* in_dev, int in_dtype, long ld_in, int x_fmt, const void* w_dev, const void* w_scale_dev, int m, int n,
                          int k, const float* bias_dev, int act, const void* resid_dev, void* out_dev, int out_dtype, void* ws_dev,
                          size_t ws_bytes, void* stream);

@@ -110,4 +110,4 @@ def test_zero_rows_launch_nothing():
     assert lib.clipenc_op_norm_quant_mx(None, 0, 0, 64, 64, None, 0, 0, None, None, 1e-6, 1, None, None, None, None) == 0
     assert lib.clipenc_op_gemm_mx(None, None, 1, None, None, 0, 8, 64, None, -1, None, None, 0, None) == 0
     assert lib.clipenc_op_linear_mx(None, 0, 64, 1, None, None, 0, 8, 64, None, -1, None, None, 0, None, 0, None) == 0
-    assert lib.clipenc_op_linear_mx_ws_bytes(0, 64, 1) == 0 and lib.clipenc_op_linear_mx_ws_bytes(400, 64, 1) >= 400 * (64 + 2)
+    assert lib.clipenc_op_linear_mx_ws_bytes(0, 8, 64, 1) == 0 and lib.clipenc_op_linear_mx_ws_bytes(400, 8, 64, 1) >= 400 * (64 + 2)
