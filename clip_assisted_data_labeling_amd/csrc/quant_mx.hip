@@ -210,8 +210,16 @@ __global__ __launch_bounds__(256) void mx_dequant_kernel(const uint8_t* __restri
 //   LAYER: the same of h - mean(h);  then y in blocks, or in e4m3 with one scale a row, max|y| / 448
 // The row stays in the registers of NT threads, CH chunks of 8 columns each, and so does its share of gamma; the next row's loads are
 // under way while a row is worked on.  Sums, the factor and y are formed in 64 bits, so that no square overflows and beta may cancel; y
-// is rounded to fp32 and from there to its few bits: a value within 2^-24 of a border between two codes may take either.
-// 65 536 rows of 1024, bf16, with residual and h: 470 MB in 92 us (5.1 TB/s, what a copy reaches); of 1280 without: 254 MB in 68 us.
+// reaches its few bits through an fp32 value rounded to ODD, so that codes are those of the 64-bit y and no value next to a border
+// between two of them is rounded twice.
+// 65 536 rows of 1024, bf16, with residual and h: 470 MB in 93 us (5.1 TB/s, what a copy reaches); of 1280 without: 254 MB in 76 us.
+__device__ __forceinline__ float to_odd(double d) {
+  // what lies below the 23 bits of an fp32 mantissa, as their last bit: the conversion has nothing left to round (normal results)
+  const uint64_t b = (uint64_t)__double_as_longlong(d);
+  const uint32_t lo = (uint32_t)b, sticky = (lo & 0x1fffffffu) + 0x1fffffffu;
+  return (float)__longlong_as_double((long long)((b >> 32 << 32) | ((lo | sticky) & 0xe0000000u)));
+}
+
 template <int NT>
 __device__ __forceinline__ double sum_over(double v, double* red) {
 #pragma unroll
@@ -346,7 +354,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void mx_norm_kernel(const MxNo
         y_of(i, y);
         float f[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = (float)(y[j] * inv);
+        for (int j = 0; j < 8; ++j) f[j] = to_odd(y[j] * inv);
         u32x2_t w = mx_to_e4m3(f, 1.0f);
         if (!fine) w = u32x2_t{0u, 0u};
         if (c < p.kp) *(u32x2_t*)(p.q + (size_t)row * p.kp + c) = w;
@@ -360,7 +368,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void mx_norm_kernel(const MxNo
         y_of(i, y);
         float f[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) f[j] = (float)y[j];
+        for (int j = 0; j < 8; ++j) f[j] = to_odd(y[j]);
         if (c < p.kp) store_block(f, p.fmt, p.q + (size_t)row * q_ld, (uint8_t*)p.scale + (size_t)row * (p.kp / 32), c);
       }
     }
@@ -400,9 +408,9 @@ void launch_dequant(const uint8_t* q, const void* scale, int fmt, long n_rows, i
 #undef DEQUANT_LAUNCH
 }
 
-// Threads of a row: as few as hold it in 24 .. 32 values each, since every wave more costs a turn of the sums (65 536 rows of 1280 / 2048 / 4096 /
-// 8192, bf16 to e4m3: 68 / 105 / 194 / 354 us; in 256 / 256 / 512 / 1024 threads of 8 values 104 / 118 / 276 / 605; 512 columns as 64 x 8 35
-// us, as 256 x 8 97).  Up to NORM_FEW rows of up to 2048 the latency of one row counts: 256 threads of 8 values (one row of 1280 3.8 us instead
+// Threads of a row: as few as hold it in 16 .. 32 values each, since every wave more costs a turn of the sums (65 536 rows of 1280 / 2048 / 4096 /
+// 8192, bf16 to e4m3: 76 / 118 / 212 / 387 us; in 256 / 256 / 512 / 1024 threads of 8 values 8 to 70 % more; 512 columns in 64 threads 36
+// us, in 256 97).  Up to NORM_FEW rows of up to 2048 the latency of one row counts: 256 threads of 8 values (one row of 1280 3.8 us instead
 // of 4.4, 1024 rows 5.3 both, 2048 rows 7.3 instead of 6.1).
 constexpr long NORM_FEW = 1024;
 template <typename T, bool WHOLE>

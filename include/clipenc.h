@@ -375,7 +375,7 @@ int clipenc_op_dequant_mx(const void* q_dev, const void* scale_dev, int fmt, lon
  *       (h - mean(h)) * gamma / sqrt(var(h) + eps) + beta           CLIPENC_NORM_LAYER       (beta_dev may be NULL)
  * and y in fmt (any of the three).  gamma / beta: float [k]; k <= 16384; ld_in / ld_resid in elements; h_out_dev may be in_dev or
  * resid_dev where that one's rows are k elements apart.  Sums, the row's factor and y are formed
- * in 64 bits; y is rounded to fp32 once, then to its few. */
+ * in 64 bits and y is rounded once, to its few (beyond fp32's range: not finite). */
 int clipenc_op_norm_quant_mx(const void* in_dev, int in_dtype, long n_rows, int k, long ld_in, const void* resid_dev, long ld_resid, int norm,
                              const float* gamma_dev, const float* beta_dev, float eps, int fmt, void* h_out_dev, void* out_dev,
                              void* scale_dev, void* stream);
