@@ -139,9 +139,8 @@ class Feature_Dataset:
         self.gpu_decode_read_ahead_bytes = 2 << 30          # file bytes the reader pool may hold ahead of the decoder
         self.pt_writers = 1                                 # threads writing the per-image .pt files of a batch (pickling holds the GIL:
                                                             # 2 and 4 measured slower than 1 next to the stager thread, tools/ab_embed_e2e.py)
-        # where the stager's decode + crop kernels go: "priority" = a high-priority stream (they start at the next boundary
-        # between two of the encoder's kernels), "side" = an ordinary second stream, "same" = the encoder's own stream
-        self.gpu_decode_stream = "priority"
+        # where the stager's decode + crop kernels go: "side" = a second stream, "same" = the encoder's own stream
+        self.gpu_decode_stream = "side"
         self.gpu_decode_queue = 6                           # encode batches the stager may be ahead of the encoder
         self.first_chunk_div = 4                            # the first decode chunk is batch_size / this many files
         # Progressive files: the device takes them, but walks each with ONE lane (scans are serial), 0.25 - 0.5 s for a chunk
@@ -332,14 +331,11 @@ class Feature_Dataset:
                     print(f"Error loading or processing image {path}: {e}")
                     return None, 0
 
-            # The stager's decode and crop kernels go to a HIGH-PRIORITY stream: they are placed at the next boundary between two of the
-            # encoder's kernels and then have the GPU to themselves for their few milliseconds.  On an ordinary second stream they
-            # only found CUs in the encoder's tail rounds -- its persistent kernels hold every CU -- and a 10-ms entropy workgroup
-            # that got one kept the next persistent kernel waiting for that CU; in the encoder's own stream the decode's final
-            # synchronisation waits for the whole batch queued before it, so the stager is never more than one batch ahead.
+            # The stager's decode and crop kernels go to a second stream, of the same priority as every other one: work on streams of
+            # different priorities can hang for good.  In the encoder's own stream the decode's final synchronisation waits for the whole
+            # batch queued before it, so the stager is never more than one batch ahead.
             mode = self.gpu_decode_stream
-            side = (torch.cuda.current_stream(self.device) if mode == "same" else
-                    torch.cuda.Stream(device=self.device, priority=-1 if mode == "priority" else 0))
+            side = torch.cuda.current_stream(self.device) if mode == "same" else torch.cuda.Stream(device=self.device)
             in_q: "queue.Queue" = queue.Queue(maxsize=int(self.gpu_decode_queue))
             stop = threading.Event()
 
