@@ -1365,7 +1365,7 @@ namespace {
 bool aligned_to(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 size_t dt_size(int dtype) { return dtype == CLIPENC_DT_F32 ? 4 : 2; }
 bool dt_known(int dtype) { return dtype == CLIPENC_DT_BF16 || dtype == CLIPENC_DT_F16 || dtype == CLIPENC_DT_F32; }
-constexpr int MX_MAX_K = 1 << 20;
+constexpr int MX_MAX_K = 1 << 20, MX_MAX_ROWS = 1 << 30;
 
 int mx_check_rows(const char* what, const void* in, int dtype, long n_rows, int k, long ld) {
   if (n_rows < 0 || k < 1 || k > MX_MAX_K) return fail("%s: %ld rows of %d columns (k = 1 .. %d)", what, n_rows, k, MX_MAX_K);
@@ -1382,7 +1382,8 @@ int mx_check_q(const char* what, const void* q, const void* scale) {
 }
 int mx_check_product(const char* what, const void* w, const void* w_scale, int m, int n, int k, const float* bias, int act, const void* resid,
                      const void* out, int out_dtype) {
-  if (m < 0 || n < 0 || k < 1 || k > MX_MAX_K) return fail("%s: bad shape m=%d n=%d k=%d (k = 1 .. %d)", what, m, n, k, MX_MAX_K);
+  if (m < 0 || n < 0 || m > MX_MAX_ROWS || n > MX_MAX_ROWS || k < 1 || k > MX_MAX_K)
+    return fail("%s: bad shape m=%d n=%d k=%d (m and n at most %d, k = 1 .. %d)", what, m, n, k, MX_MAX_ROWS, MX_MAX_K);
   if (!dt_known(out_dtype)) return fail("%s: out_dtype = %d (CLIPENC_DT_*)", what, out_dtype);
   if (act != -1 && act != CLIPENC_ACT_QUICK_GELU && act != CLIPENC_ACT_GELU_ERF) return fail("%s: act = %d", what, act);
   if (resid && act != -1) return fail("%s: activation and residual are exclusive", what);

@@ -21,6 +21,7 @@ NORMS = {"rms": 0, "layer": 1}
 ACTS = {None: -1, "quick_gelu": 0, "gelu": 1}
 _BLOCKS = {"e2m1": 0, "e4m3": 1}      # formats of a product's rows
 _WEIGHTS = {"e2m1": 0}                # and of its weights
+_MAX_ROWS = 1 << 30
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
@@ -192,6 +193,8 @@ def linear(x, w: MXTensor, bias: Optional[torch.Tensor] = None, act: Optional[st
         if fmt is None:
             raise ValueError(f"{what}: x_fmt must be 'e2m1' or 'e4m3', got {x_fmt!r}")
         dt, x_index, rows, cols, ld = _check_values(what, x)
+    if rows > _MAX_ROWS or n > _MAX_ROWS:
+        raise ValueError(f"{what}: at most {_MAX_ROWS} rows of x and of w, got {rows} and {n}")
     if x_index != index or cols != w_cols:
         raise ValueError(f"{what}: x has {cols} columns on cuda:{x_index} and w {w_cols} on cuda:{index}")
     if out_dtype is None:

@@ -354,7 +354,8 @@ int clipenc_op_gemm_fp8_resid_q(const void* a8_dev, const void* w8_dev, int m, i
  *             0xff: the block held an infinity or a NaN and is NaN
  * elements are v / 2^X rounded to nearest (ties to even), at most 6 / 448.  CLIPENC_ROW_E4M3: kp e4m3 bytes a row and ONE float scale a
  * row, max|v| / 448 (0 for a zero row, NaN for one that is not finite): what clipenc_op_gemm_fp8 takes as scale_a where k % 256 == 0.
- * All matrices are row-major; elements 16-byte aligned, scale bytes 4-byte aligned, values aligned to their type only; 1 <= k <= 2^20.
+ * All matrices are row-major; elements 16-byte aligned, scale bytes 4-byte aligned, values aligned to their type only; 1 <= k <= 2^20, and of a
+ * product m, n <= 2^30.
  * Nothing is read or written behind the last row; zero rows (n_rows, m or n = 0) are a call that does nothing.  Every call is
  * deterministic, needs no scratch but what it names, and may be captured into a graph. */
 #define CLIPENC_DT_F32 2

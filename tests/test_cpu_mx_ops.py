@@ -111,3 +111,17 @@ def test_zero_rows_launch_nothing():
     assert lib.clipenc_op_gemm_mx(None, None, 1, None, None, 0, 8, 64, None, -1, None, None, 0, None) == 0
     assert lib.clipenc_op_linear_mx(None, 0, 64, 1, None, None, 0, 8, 64, None, -1, None, None, 0, None, 0, None) == 0
     assert lib.clipenc_op_linear_mx_ws_bytes(0, 8, 64, 1) == 0 and lib.clipenc_op_linear_mx_ws_bytes(400, 8, 64, 1) >= 400 * (64 + 2)
+
+
+@pytest.mark.parametrize("change", [dict(m=(1 << 30) + 1), dict(n=(1 << 30) + 1)])
+def test_linear_refuses_more_rows_than_its_indices_hold(change):
+    _refused("clipenc_op_linear_mx", *_linear(**change), match="at most")
+
+
+@pytest.mark.parametrize("rows,out", [((1 << 30) + 1, 4), (3, (1 << 32) + 3)])
+def test_the_wrapper_refuses_more_rows_than_an_int_holds(monkeypatch, rows, out):
+    checked = iter([(0, 0, out, 64), (1, 0, rows, 64)])
+    monkeypatch.setattr(mx, "_check_quantised", lambda *a: next(checked))
+    q = mx.MXTensor(None, None, "e4m3", 64)
+    with pytest.raises(ValueError, match="at most"):
+        mx.linear(q, q)

@@ -12,6 +12,9 @@ Tolerances, u = 2^-24 (half a step of fp32):
                          exponent of the smallest normal number): together less than 2^(E - 10), at most 2^-10 max 2^ea max 2^ew
 """
 import ctypes
+import subprocess
+import sys
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -168,6 +171,13 @@ def test_norm_quantize(gpu, rows, cols, dtype, norm, bias, residual, fmt):
     assert torch.equal(h.cpu(), want_h)
     y = ora.norm(_np(want_h), _np(w), _np(b) if bias else None, norm, float(np.float32(1e-5)))
     _check_codes(q, y)
+
+
+@pytest.mark.parametrize("fmt", ["e2m1", "e4m3", "e4m3_row"])
+@pytest.mark.parametrize("norm,bias,residual", [("rms", False, True), ("layer", True, False)])
+@pytest.mark.parametrize("rows,cols,dtype", [(1100, 1500, torch.bfloat16), (1025, 1304, torch.float32), (1031, 2000, torch.float16), (1040, 1537, torch.float32), (2100, 2048, torch.bfloat16)])
+def test_norm_quantize_many_rows(gpu, rows, cols, dtype, norm, bias, residual, fmt):
+    test_norm_quantize(gpu, rows, cols, dtype, norm, bias, residual, fmt)
 
 
 @pytest.mark.parametrize("fmt", ["e2m1", "e4m3", "e4m3_row"])
@@ -329,6 +339,50 @@ def test_linear_of_values_is_quantize_and_linear(gpu, m, n, k, dtype, fmt):
     cut = _linear_cut(q, w, dtype)
     _check_linear(y, a, wv, None, None, None, dtype, cut)
     _check_linear(mx.linear(q, w, out_dtype=dtype), a, wv, None, None, None, dtype, cut)
+
+
+@pytest.mark.parametrize("fmt", ["e2m1", "e4m3"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k", [(1, 8193, 200), (16, 9001, 300), (3, 33000, 128), (2, 16400, 4095), (60, 100, 700), (49, 2049, 130), (5000, 40, 77), (16000, 16, 130)])
+def test_linear_of_values_few_rows_or_few_columns(gpu, m, n, k, dtype, fmt):
+    """Rows quantised inside and in front of the product, one and four column fragments a workgroup, more weights than are swept with it."""
+    x = _rows(m, k, k, dtype, 0.5)
+    w, wv = _random_coded(n, k, "e2m1", 7, gpu)
+    q = mx.quantize(x.to(gpu), fmt)
+    a = ora.values(_codes(q), q.scale.cpu().numpy(), fmt, k)
+    cut = _linear_cut(q, w, dtype)
+    _check_linear(mx.linear(x.to(gpu), w, x_fmt=fmt), a, wv, None, None, None, dtype, cut)
+    _check_linear(mx.linear(q, w, out_dtype=dtype), a, wv, None, None, None, dtype, cut)
+
+
+def test_first_calls_inside_a_capture(gpu):
+    """A process whose first call of each kernel is captured: nothing in it may synchronise."""
+    code = """
+import torch
+from clip_assisted_data_labeling_amd import mx_ops as mx
+torch.manual_seed(1)
+x = torch.randn(4200, 1600, device="cuda", dtype=torch.bfloat16)
+wt = torch.randn(4100, 1600, device="cuda")
+gamma = torch.ones(1600, device="cuda")
+torch.cuda.synchronize()
+
+def chain(rows):
+    w = mx.quantize(wt)
+    h, q = mx.norm_quantize(x[:rows], gamma, residual=x[:rows])
+    return mx.linear(q, w), mx.linear(h, w, x_fmt="e2m1"), mx.dequantize(q)
+
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = [chain(rows) for rows in (3, 70, 300, 4200)]
+for _ in range(2):
+    graph.replay()
+    torch.cuda.synchronize()
+    for got, rows in zip(out, (3, 70, 300, 4200)):
+        assert all(torch.equal(a, b) for a, b in zip(got, chain(rows))), rows
+print("equal")
+"""
+    done = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=100, cwd=str(Path(__file__).resolve().parents[1]))
+    assert done.returncode == 0 and done.stdout.strip().endswith("equal"), done.stderr[-2000:]
 
 
 @pytest.mark.parametrize("m", [1, 5, 40, 300])
