@@ -23,6 +23,11 @@
 // with both scales at 2^-127: products below 2^-240, zeros in fp32.
 // Scales come by periods of 512 columns, the four words of a row turned round -- word g: the scales of block g in the period's four K
 // steps -- so that a lane holds the scales of 16 rows and a period in ONE word.
+//
+// Measured, 256 x 256 tiles:  16 384 x 8192 -> 4096  e2m1 271 us (4.05 PFLOP/s), e4m3 382 us (2.9);  65 536 x 4096 -> 1024  160 us (3.4),
+// 221 us (2.5); the bare instruction reaches 7.7 and 4.5.  An e4m3 stage of 128 columns takes 4100 cycles where its products take 2048: 48
+// KiB through the vector memory path (16 cycles a KiB) and 160 KiB of fragments out of LDS, in turns with the products as far as they
+// go.  A short K is bound by the way out: 65 792 x 1024 -> 4096 with QuickGELU 253 us, 539 MB of results.
 #include <type_traits>
 
 #include "common.h"
