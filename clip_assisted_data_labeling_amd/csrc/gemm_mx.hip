@@ -9,9 +9,9 @@
 //
 // What the matrix pipe keeps (measured): the products of 8 neighbouring columns are added at fixed point, cut below 2^(E - 13), 2^E the
 // largest product's power of two; everything above that is added in fp32.  e2m1 products span 6 bits and lose nothing.  e4m3 x e2m1
-// products span 22: on quantised normal rows 1.2e-5 of the result, without bias, where bf16 rounds at 1.7e-3 and fp16 at 2e-4 -- taken
-// for 16-bit results.  An fp32 result gets the sum in two BANDS of e4m3 codes, exponent fields 8 .. 15 and 0 .. 7: a band's products span
-// at most 14 bits (2^-3 .. 2^11, 2^-10 .. 2^3), so nothing is cut, at two MFMAs a fragment pair.
+// products span 22, so that two large ones of opposite signs among eight neighbours would leave nothing of the six others.  They are
+// therefore added in two BANDS of the e4m3 codes, exponent fields 8 .. 15 and 0 .. 7: a band's products span at most 14 bits (2^-3 .. 2^11,
+// 2^-10 .. 2^3), so nothing is cut, at two MFMAs a fragment pair.
 //
 // Persistent tiles of BM x BN, WM x WN waves.  LDS holds two stages of 128-byte rows of A (256 columns of e2m1, 128 of e4m3) and two of W
 // (256 columns), brought in by LDS-DMA in pieces of 8 rows x 128 bytes.  The walk is one sequence of stages over all of a workgroup's
@@ -24,10 +24,10 @@
 // Scales come by periods of 512 columns, the four words of a row turned round -- word g: the scales of block g in the period's four K
 // steps -- so that a lane holds the scales of 16 rows and a period in ONE word.
 //
-// Measured, 256 x 256 tiles:  16 384 x 8192 -> 4096  e2m1 271 us (4.05 PFLOP/s), e4m3 382 us (2.9);  65 536 x 4096 -> 1024  160 us (3.4),
-// 221 us (2.5); the bare instruction reaches 7.7 and 4.5.  An e4m3 stage of 128 columns takes 4100 cycles where its products take 2048: 48
-// KiB through the vector memory path (16 cycles a KiB) and 160 KiB of fragments out of LDS, in turns with the products as far as they
-// go.  A short K is bound by the way out: 65 792 x 1024 -> 4096 with QuickGELU 253 us, 539 MB of results.
+// Measured, 256 x 256 tiles:  16 384 x 8192 -> 4096  e2m1 271 us (4.05 PFLOP/s), e4m3 784 us (1.4, of MFMAs in two bands 2.8);  65 536 x 4096
+// -> 1024 in e2m1 160 us (3.4), 65 792 in e4m3 434 us (1.27); the bare instruction reaches 7.7 and 4.5.  Long e4m3 rows are bound by the
+// matrix pipe (one MFMA a fragment pair, whose sums the cut above would hold in 14 bits: 402 and 242 us).  A short K is bound by the way
+// out: 65 792 x 1024 -> 4096 in e2m1 with QuickGELU 253 us, 539 MB of results.
 #include <type_traits>
 
 #include "common.h"
@@ -35,7 +35,7 @@
 
 namespace {
 
-enum { A_E2M1 = 0, A_E4M3 = 1, A_E4M3_BANDS = 2 };   // the kernels' A
+enum { A_E2M1 = 0, A_E4M3 = 1 };   // the kernels' A
 
 typedef __attribute__((ext_vector_type(4))) int i32x4_t;
 typedef __attribute__((ext_vector_type(8))) int i32x8_t;
@@ -152,8 +152,8 @@ __device__ __forceinline__ void for_each_int(F&& f) {
 }
 
 // NS: stages of A in LDS, NS - 1 of them under way.  DIRECT: scales come with each stage, a word a row and K step, and lanes read their byte
-// of it; else by periods, turned.  PAIRED: the two rows of waves in turns.
-template <int AF, int BM_, int BN_, int WM_, int WN_, int NS_, bool DIRECT_, bool PAIRED_>
+// of it; else by periods, turned.
+template <int AF, int BM_, int BN_, int WM_, int WN_, int NS_, bool DIRECT_>
 struct Tile {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
   static constexpr int NS = NS_, NB = NS + 1;                      // NB: biases held -- a tile may be one stage, and that many are under way
@@ -171,14 +171,13 @@ struct Tile {
   static_assert(A_PER >= W_PER && FM >= 2 && FN % 2 == 0 && A_PER * NW * 8 == BM && W_PER * NW * 8 == BN && NW % 2 == 0, "pieces");
   static_assert(BM % 64 == 0 && NS >= 2 && YOUNGER + STORES < 64, "ring");
   static_assert(DIRECT || NS == 2, "turned scales are one stage ahead");
-  static_assert(!PAIRED_ || (AF == A_E4M3 && !DIRECT && WM == 2 && BM == BN && BN / 64 == WN && WN % 2 == 0), "turns");
   static_assert(SC_PER * THREADS == SC_ROWS * 4 && BM % (THREADS / 4) == 0 && BN % 64 == 0 && BN <= THREADS, "scales, bias");
   static_assert(LDS <= 163840, "LDS");
 };
 
-template <int AF, int BM, int BN, int WM, int WN, int NS, bool DIRECT, bool PAIRED = false>
+template <int AF, int BM, int BN, int WM, int WN, int NS, bool DIRECT>
 __global__ __launch_bounds__(WM * WN * 64, 2) void mx_gemm_kernel(const MxGemmParams p) {
-  using T = Tile<AF, BM, BN, WM, WN, NS, DIRECT, PAIRED>;
+  using T = Tile<AF, BM, BN, WM, WN, NS, DIRECT>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -306,7 +305,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mx_gemm_kernel(const MxGemmPa
     f_sa = uniform(p.a_scale + ((long)f_m0 * s_ld - odd * 4));
     f_sw = uniform(p.w_scale + ((long)f_n0 * s_ld - odd * 4));
   };
-  if constexpr (!PAIRED) fetch_tile();
+  fetch_tile();
   auto fetch = [&]() {
     f_period = -1;
     if (f_idx >= nwg) return;
@@ -431,126 +430,6 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mx_gemm_kernel(const MxGemmPa
     }
   };
 
-  if constexpr (PAIRED) {
-    // The two rows of waves in turns: one reads a K step's fragments into registers and asks for rows to come, the other -- on the same
-    // SIMDs -- multiplies.  ROW 0 brings A, a K step ahead; ROW 1, half a step behind, brings W, a pair of steps ahead.  Step s is read in
-    // phase 2 s by ROW 0 and in phase 2 s + 1 by ROW 1, so its buffer is free from phase 2 s + 2 on, where ROW 0 asks for step s + 2; that
-    // has to be there by phase 2 s + 4, and ROW 0 waits for it behind its products of phase 2 s + 3.  W and, with the pairs of steps, its
-    // scales are waited for by ROW 1 where a pair is read for the last time.  A finished tile's results leave at the start of a phase,
-    // behind the asking, so that they may stay behind it (wait_stage).  Both rows pass 2 steps + 2 barriers.
-    auto turns = [&](auto row_) __attribute__((always_inline)) {
-      constexpr int ROW = decltype(row_)::value;
-      constexpr int ROWS = ROW == 0 ? BM : BN, PIECES = ROWS / 8 / WN, BUFFER = ROWS * 128;
-      const unsigned ld = ROW == 0 ? a_ld : w_ld;
-      unsigned off = (unsigned)((w % WN) * 8 + lr) * ld;
-      const unsigned to = __builtin_amdgcn_readfirstlane(lds0 + (unsigned)((ROW == 0 ? 0 : T::W_OFF) + (w % WN) * 1024));
-      auto ask_tile = [&]() __attribute__((always_inline)) {
-        tile_at(f_idx, f_m0, f_n0);
-        f_v = v0;
-        f_a = uniform(ROW == 0 ? p.a + (long)f_m0 * a_ld : p.w + ((long)f_n0 * w_ld - odd * 64));
-        f_sa = uniform(p.a_scale + ((long)f_m0 * s_ld - odd * 4));
-        f_sw = uniform(p.w_scale + ((long)f_n0 * s_ld - odd * 4));
-      };
-      auto ask = [&]() __attribute__((always_inline)) {
-        f_period = -1;
-        if (f_idx >= nwg) return;
-        const bool first = f_v == v0;
-        asm volatile("" : "+v"(off));                // its sums are worked out here, not held in registers
-        const unsigned plus = low + (ROW == 1 && first && odd ? lead : 0u);
-        const unsigned last = (unsigned)min(ROW == 0 ? p.M - 1 - f_m0 : p.N - 1 - f_n0, ROWS - 1) * ld;
-#pragma unroll
-        for (int i = 0; i < PIECES; ++i) dma16(f_a, min(off + (unsigned)(i * WN * 8) * ld, last) + plus, to + (unsigned)(f_ab * BUFFER + i * WN * 1024));
-        f_a += 128;
-        f_ab = after(f_ab, NS);
-        if ((f_v & 3) == 0 || first) {
-          f_period = f_v >> 2;
-          issue_scales(f_sa, f_sw, p.M - f_m0, p.N - f_n0, f_period);
-          f_sa += 16;
-          f_sw += 16;
-        }
-        if (ROW == 0 && first) {
-          if (p.bias) dma4((const uint8_t*)p.bias, (unsigned)min(f_n0 + tid, p.N - 1) * 4u, lds0 + (unsigned)(T::BIAS_OFF + f_bias * BN * 4 + w * 256));
-          f_bias = after(f_bias, T::NB);
-        }
-        f_v += ROW == 0 ? 1 : 2 - (f_v & 1);
-        if (f_v >= steps) {
-          f_idx += (int)gridDim.x;
-          if (f_idx < nwg) ask_tile();
-        }
-      };
-      auto wait = [&]() __attribute__((always_inline)) {
-        wait_stage(stored);
-        stored = false;
-        if (f_period >= 0) turn_scales(f_period, sb ^ 1);
-      };
-      ask_tile();
-      ask();
-      WAIT_ALL();
-      turn_scales(0, 0);
-      WAIT_LDS();
-      BARRIER();
-      if (ROW == 1) BARRIER();                       // half a step behind
-      bool asked = false;                            // in front of the results
-      i32x8_t wf[FN], af[FM];
-      uint32_t sa[FM], sw[FN];
-      while (true) {
-#pragma unroll
-        for (int i = 0; i < FM; ++i)
-#pragma unroll
-          for (int j = 0; j < FN; ++j) acc[i][j] = f32x4_t{0, 0, 0, 0};
-        int v = v0;
-        bool last;
-#pragma clang loop unroll(disable)
-        do {
-          const bool opens = (v & 1) == 0 || v == v0, closes = (v & 1) != 0;       // its pair of steps
-#pragma unroll
-          for (int j = 0; j < FN; ++j) sw[j] = load_scale(sb, v & 3, 0, FM * WM + wn * FN + j);
-#pragma unroll
-          for (int i = 0; i < FM; ++i) sa[i] = load_scale(sb, v & 3, 0, wm * FM + i);
-#pragma unroll
-          for (int j = 0; j < FN; ++j) wf[j] = load_w(wb, v & 3, 0, j);
-#pragma unroll
-          for (int i = 0; i < FM; ++i) af[i] = load_a(ab, 0, i);
-          if (!asked && (ROW == 0 || opens)) ask();
-          asked = asked && ROW == 1 && !closes;
-          if (ROW == 1 && closes) wait();
-          WAIT_LDS();
-          BARRIER();
-#pragma unroll
-          for (int i = 0; i < FM; ++i) {
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int j = 0; j < FN; ++j)
-              acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[j], af[i], acc[i][j], 4, 0, 0, (int)sw[j], 0, (int)sa[i]);
-            __builtin_amdgcn_sched_barrier(0);
-          }
-#pragma unroll
-          for (int i = 0; i < FM; ++i)
-#pragma unroll
-            for (int j = 0; j < FN; ++j) asm volatile("" : "+v"(acc[i][j]));   // the products stay in front of the wait (no instruction)
-          if (ROW == 0) wait();
-          WAIT_LDS();
-          BARRIER();
-          last = v + 1 >= steps;
-          ab = after(ab, NS);
-          if (closes) wb = after(wb, NS);
-          if ((v & 3) == 3 || last) sb ^= 1;
-          ++v;
-        } while (!last);
-        ask();
-        asked = true;
-        results();
-        bias_buf = after(bias_buf, T::NB);
-        idx += (int)gridDim.x;
-        if (idx >= nwg) break;
-        tile_at(idx, m0, n0);
-      }
-      if (ROW == 0) BARRIER();
-    };
-    if (wm == 0) turns(std::integral_constant<int, 0>{});
-    else turns(std::integral_constant<int, 1>{});
-    return;
-  }
 #pragma unroll
   for (int i = 0; i < NS - 1; ++i) fetch();
   wait_stage(false);
@@ -586,7 +465,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mx_gemm_kernel(const MxGemmPa
         i32x8_t a = af[t % 3];
         const int s = (int)sa[t % 3];
         constexpr int OP = DIRECT ? 0 : step;
-        if constexpr (AF == A_E4M3_BANDS) {
+        if constexpr (AF == A_E4M3) {
           const i32x8_t high = high_band(a);
           a ^= high;
 #pragma unroll
@@ -798,7 +677,7 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void mx_few_kernel(const MxFewParam
 #pragma unroll
       for (int i = 0; i < MF; ++i) {
         i32x8_t a = af[u][i];
-        if constexpr (AF == A_E4M3_BANDS) {
+        if constexpr (AF == A_E4M3) {
           const i32x8_t high = high_band(a);
           a ^= high;
 #pragma unroll
@@ -850,29 +729,29 @@ hipError_t launch_few(const MxFewParams& p, hipStream_t stream) {
   return per >= 2 ? launch_few_u<T, AF, MF, NF, 2>(p, stream) : launch_few_u<T, AF, MF, NF, 1>(p, stream);
 }
 
-template <int AF, int BM, int BN, int WM, int WN, int NS, bool DIRECT, bool PAIRED = false>
+template <int AF, int BM, int BN, int WM, int WN, int NS, bool DIRECT>
 hipError_t launch(const MxGemmParams& p, hipStream_t stream) {
-  using T = Tile<AF, BM, BN, WM, WN, NS, DIRECT, PAIRED>;
+  using T = Tile<AF, BM, BN, WM, WN, NS, DIRECT>;
   static DeviceKernelSetup setup;
   int n_cu = 0;
-  if (hipError_t e = setup.ensure((const void*)mx_gemm_kernel<AF, BM, BN, WM, WN, NS, DIRECT, PAIRED>, T::LDS, &n_cu); e != hipSuccess) return e;
+  if (hipError_t e = setup.ensure((const void*)mx_gemm_kernel<AF, BM, BN, WM, WN, NS, DIRECT>, T::LDS, &n_cu); e != hipSuccess) return e;
   const long tiles = (long)((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN);
   if (tiles > 0x3fffffff) return hipErrorInvalidValue;
   const long resident = (long)n_cu * (163840 / T::LDS);             // workgroups that the CUs hold
-  hipLaunchKernelGGL((mx_gemm_kernel<AF, BM, BN, WM, WN, NS, DIRECT, PAIRED>), dim3((unsigned)(tiles < resident ? tiles : resident)), dim3(T::THREADS), T::LDS, stream, p);
+  hipLaunchKernelGGL((mx_gemm_kernel<AF, BM, BN, WM, WN, NS, DIRECT>), dim3((unsigned)(tiles < resident ? tiles : resident)), dim3(T::THREADS), T::LDS, stream, p);
   return hipGetLastError();
 }
 
 // Fewer than a 256 x 256 tile a CU.  64 x 64 tiles while the CUs hold them in one go or nearly (two a CU, a third one joins late); beyond that
 // 128 x 128: 5120 columns of 577 / 1154 rows, e4m3: 19 / 25 us in 64 x 64, 15 / 17 in 128 x 128 -- in eight waves with four stages in LDS while
-// they are at most one a CU, and latency is what a stage costs, else in four waves, two workgroups a CU.  (e4m3 in bands: waves of 32 x 64, which
+// they are at most one a CU, and latency is what a stage costs, else in four waves, two workgroups a CU.  (e4m3: waves of 32 x 64, which
 // part each row fragment for four products instead of two: 46 -> 40 us at 2885 x 4001 -> 1003.)
 template <int AF>
 hipError_t small_tiles(const MxGemmParams& p, hipStream_t stream) {
   const long tiles64 = (long)((p.M + 63) / 64) * ((p.N + 63) / 64), tiles128 = (long)((p.M + 127) / 128) * ((p.N + 127) / 128);
   if (tiles64 <= 704) return launch<AF, 64, 64, 2, 2, 4, true>(p, stream);
   if (tiles128 > 256) return launch<AF, 128, 128, 2, 2, 2, false>(p, stream);
-  if constexpr (AF == A_E4M3_BANDS) return launch<AF, 128, 128, 4, 2, 4, true>(p, stream);
+  if constexpr (AF == A_E4M3) return launch<AF, 128, 128, 4, 2, 4, true>(p, stream);
   else return launch<AF, 128, 128, 2, 4, 4, true>(p, stream);
 }
 
@@ -889,13 +768,8 @@ hipError_t few_rows(const MxGemmParams& p, hipStream_t stream) {
   return p.M <= 16 ? launch_few<void, AF, 1>(f, stream) : p.M <= 32 ? launch_few<void, AF, 2>(f, stream) : launch_few<void, AF, 4>(f, stream);
 }
 
-// 256 x 256 tiles.  e4m3 rows of 12 K steps on with the rows of waves in turns, which keeps the matrix pipe busier over a long K (4096 -> 1024,
-// 65 536 rows: 258 -> 221 us) but lets half the waves wait while the others' results leave (1024 -> 4096, 16 384 rows: 75.7 -> 80.1; 1280 -> 5120:
-// 146 -> 145).  e2m1 rows, whose products are half as long, lose by it (4096 -> 1024: 160 -> 178).
 template <int AF>
 hipError_t large_tiles(const MxGemmParams& p, hipStream_t stream) {
-  if constexpr (AF == A_E4M3)
-    if (p.nk >= 12) return launch<AF, 256, 256, 2, 4, 2, false, true>(p, stream);
   return launch<AF, 256, 256, 2, 4, 2, false>(p, stream);
 }
 
@@ -928,7 +802,7 @@ hipError_t ce_mx_gemm(MxGemmParams p, int a_fmt, hipStream_t stream) {
   // panels stay (65 792 x 1024 -> 4096: 265 -> 253 us; onto a residual it costs 1 %).
   p.streamed = !p.resid && (size_t)p.M * p.N * 2 > (64u << 20);
   if (a_fmt == MX_E2M1) return choose<A_E2M1>(p, stream);
-  return p.out_dtype == MX_DT_F32 ? choose<A_E4M3_BANDS>(p, stream) : choose<A_E4M3>(p, stream);
+  return choose<A_E4M3>(p, stream);
 }
 
 template <typename T, int AF>
@@ -937,8 +811,7 @@ static hipError_t few_values_of(const MxFewParams& f, hipStream_t stream) {
 }
 template <typename T>
 static hipError_t few_values(const MxFewParams& f, int fmt, hipStream_t stream) {
-  if (fmt == MX_E2M1) return few_values_of<T, A_E2M1>(f, stream);
-  return f.g.out_dtype == MX_DT_F32 ? few_values_of<T, A_E4M3_BANDS>(f, stream) : few_values_of<T, A_E4M3>(f, stream);
+  return fmt == MX_E2M1 ? few_values_of<T, A_E2M1>(f, stream) : few_values_of<T, A_E4M3>(f, stream);
 }
 hipError_t ce_mx_gemm_values(const MxGemmParams& p, const void* x, int dtype, long ld_x, int k, int fmt, hipStream_t stream) {
   if (!mx_takes_values(p.M, p.N, k)) return hipErrorInvalidValue;

@@ -1,0 +1,109 @@
+"""Values of the microscaled operators where they are easily lost: sums that cancel, results of every type out of every kernel, the activations' tails,
+values next to a border between two codes, row scales, and what lies beside a result.
+
+Tolerances, u = 2^-24, half(t) = torch.finfo(t).eps / 2.
+  sums          products of e2m1 / e4m3 values and powers of two are exact in fp32; a K step of 128 adds at most 128 roundings and each further step
+                one, none larger than u times the products' magnitudes, in whatever order and for whatever type of result; then two fp32 roundings
+                (bias, residual) and one to the result's type
+  activations   of an exact argument, relative.  16-bit results: their own half step and 2^-14 (a fit good to 2^-15.1, and exp2's argument,
+                at most 128 with two roundings of u: 256 u ln 2 < 2^-16).  fp32: 16 u (exp2 and rcp 2 u each, the fit and its
+                eight steps 6 u, four products and sums 4 u; the exponential's argument is carried in two floats).  Results below 2^-120 may be
+                lost to subnormal numbers on the way
+"""
+import numpy as np
+import pytest
+import torch
+
+from clip_assisted_data_labeling_amd import _lib, mx_ops as mx
+from oracle import mx_oracle as ora
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+DTYPES = [BF16, F16, F32]
+
+
+def _half(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def _lay_out(codes, scale, fmt, cols, gpu):
+    return mx.MXTensor(torch.from_numpy(ora.pack(codes, fmt)).to(gpu), torch.from_numpy(scale).to(gpu), fmt, cols)
+
+
+def _coded(rows, cols, fmt, seed, gpu, low, high):
+    """Any codes, scales 2^low .. 2^high, zero behind the columns; and the values on the GPU in 64 bits."""
+    r = np.random.RandomState(seed)
+    kp = ora.padded(cols)
+    codes = r.randint(0, 16 if fmt == "e2m1" else 256, (rows, kp)).astype(np.uint8)
+    if fmt == "e4m3":
+        codes[(codes & 127) == 127] = 0                          # its NaN codes
+    codes[:, cols:] = 0
+    scale = r.randint(127 + low, 128 + high, (rows, kp // 32)).astype(np.uint8)
+    return _lay_out(codes, scale, fmt, cols, gpu), torch.from_numpy(ora.values(codes, scale, fmt, cols)).to(gpu)
+
+
+def _operands(m, n, k, fmt, gpu):
+    """Rows and weights whose sums are a few units wide."""
+    a, av = _coded(m, k, fmt, m + k, gpu, *((-10, -7) if fmt == "e4m3" else (-3, 0)))
+    w, wv = _coded(n, k, "e2m1", n + k, gpu, -6, -3)
+    return a, av, w, wv
+
+
+def _activate(u, act):
+    if act == "gelu":
+        return u * torch.special.erfc(-u / 2 ** 0.5) / 2
+    return u / (1 + torch.exp(-1.702 * u)) if act == "quick_gelu" else u
+
+
+def _act_error(want, dtype):
+    return (16 * U if dtype == F32 else 2.0 ** -14) * want.abs() + 2.0 ** -120
+
+
+def _check(y, u, pre, act, residual, dtype, what):
+    """u: the sums with their bias in 64 bits, good to `pre`."""
+    want = _activate(u, act)
+    tol = pre if act is None else 1.13 * pre + _act_error(want, dtype)
+    if residual is not None:
+        want = want + residual.double()
+    tol = tol + 2 * U * want.abs()
+    tol = tol + _half(dtype) * (want.abs() + tol) + float(torch.finfo(dtype).smallest_normal) * torch.finfo(dtype).eps
+    off = (y.double() - want).abs() - tol
+    assert y.dtype == dtype and y.shape == want.shape and not torch.isnan(y).any()
+    assert not (off > 0).any(), (what, off.max().item(), np.unravel_index(int(off.argmax()), tuple(off.shape)))
+
+
+# One shape or two -- whole tiles, ragged ones -- for each kernel of a product: the few-row kernel (up to 16 rows, or one or two workgroups a CU of 64 rows x 16
+# columns), 64 x 64 tiles (a few hundred), 128 x 128 in four stages (up to 256 of them), 128 x 128 in two, 256 x 256 (from 256 of them on; rows that
+# would leave a last round nearly empty go to a smaller kernel), and those of a long K
+KERNELS = {"few-1": (1, 1000, 700), "few-16": (16, 1664, 1281), "few-64": (61, 500, 1000), "few-columns": (300, 17, 600),
+           "tiles-64": (320, 1024, 384), "tiles-64-ragged": (301, 1101, 200),
+           "tiles-128-deep": (2048, 1664, 640), "tiles-128-deep-ragged": (2885, 1003, 601),
+           "tiles-128": (2816, 2944, 384), "tiles-128-ragged": (2900, 3001, 200),
+           "tiles-256": (4096, 4096, 256), "tiles-256-ragged": (5300, 4090, 300), "tiles-256-and-few": (4100, 4090, 300), "tiles-256-and-128": (11000, 1664, 130),
+           "tiles-256-long": (4096, 4096, 1664), "tiles-256-long-ragged": (5300, 4104, 1801)}
+
+
+# ------------------------------------------------------------------------------------------ sums
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_sums_of_e4m3_rows_whose_large_products_cancel(gpu, kernel, dtype):
+    """Two of eight neighbouring columns hold +-448 against the same weight 6, the six others make the result."""
+    m, n, k = KERNELS[kernel]
+    k = ora.padded(k)
+    r = np.random.RandomState(m)
+    codes = (0x10 + r.randint(0, 8, (m, k))).astype(np.uint8)                     # 2^-5 .. 2^-4, positive
+    codes[:, 2::8], codes[:, 5::8] = 0x7E, 0xFE                                   # +-448
+    wcodes = r.randint(2, 4, (n, k)).astype(np.uint8)                             # 1, 1.5
+    wcodes[:, 2::8] = wcodes[:, 5::8] = 7                                         # 6
+    ones = lambda rows: np.full((rows, k // 32), 127, np.uint8)                   # noqa: E731
+    a, w = _lay_out(codes, ones(m), "e4m3", k, gpu), _lay_out(wcodes, ones(n), "e2m1", k, gpu)
+    av, wv = (torch.from_numpy(ora.values(c, s, f, k)).to(gpu) for c, s, f in ((codes, ones(m), "e4m3"), (wcodes, ones(n), "e2m1")))
+    u, size = av @ wv.t().contiguous(), av.abs() @ wv.abs().t().contiguous()
+    y = mx.linear(a, w, out_dtype=dtype)
+    _check(y, u, (128 + k // 128) * U * size, None, None, dtype, kernel)
+    if m <= 16:                                                                   # and from values, which are these codes
+        x = av.to(F32)
+        assert torch.equal(mx.dequantize(mx.quantize(x, "e4m3"), F32), x)
+        _check(mx.linear(x, w, out_dtype=dtype), u, (128 + k // 128) * U * size, None, None, dtype, kernel)
