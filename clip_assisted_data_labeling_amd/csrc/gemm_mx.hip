@@ -625,7 +625,8 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void mx_few_kernel(const MxFewParam
   __shared__ __attribute__((aligned(16))) float sums[FEW_WAVES][MF * NF][256];
   const int tid = threadIdx.x, lane = tid & 63, r16 = lane & 15, g = lane >> 4;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6), waves = blockDim.x >> 6;
-  const int n0 = blockIdx.x * (NF * 16), m0 = blockIdx.y * (MF * 16);
+  const int n0 = (blockIdx.z * gridDim.x + blockIdx.x) * (NF * 16), m0 = blockIdx.y * (MF * 16);
+  if (n0 >= p.N) return;                                                           // (the whole workgroup)
   size_t w_row[NF], a_row[MF];                                                     // in K steps
 #pragma unroll
   for (int j = 0; j < NF; ++j) w_row[j] = (size_t)min(n0 + j * 16 + r16, p.N - 1) * p.nk;
@@ -713,10 +714,14 @@ __global__ __launch_bounds__(FEW_WAVES * 64) void mx_few_kernel(const MxFewParam
   }
 }
 
+// A dimension of a launch holds fewer than 2^32 work items -- 2^23 workgroups of 512, 2^27 columns in 16s --, and more are cut off without an
+// error: beyond FEW_COLUMNS workgroups the columns go on in the grid's third dimension (2^30 of them: 16 rows of it).
+constexpr unsigned FEW_COLUMNS = 1u << 22;
 template <typename T, int AF, int MF, int NF, int U>
 hipError_t launch_few_u(const MxFewParams& p, hipStream_t stream) {
   const int waves = p.g.nk < FEW_WAVES ? p.g.nk : FEW_WAVES;
-  const dim3 grid((unsigned)((p.g.N + NF * 16 - 1) / (NF * 16)), (unsigned)((p.g.M + MF * 16 - 1) / (MF * 16)));
+  const unsigned cols = (unsigned)((p.g.N + NF * 16 - 1) / (NF * 16)), x = cols < FEW_COLUMNS ? cols : FEW_COLUMNS;
+  const dim3 grid(x, (unsigned)((p.g.M + MF * 16 - 1) / (MF * 16)), (cols + x - 1) / x);
   hipLaunchKernelGGL((mx_few_kernel<T, AF, MF, NF, U>), grid, dim3((unsigned)waves * 64), 0, stream, p);
   return hipGetLastError();
 }

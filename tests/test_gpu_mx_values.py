@@ -107,3 +107,24 @@ def test_sums_of_e4m3_rows_whose_large_products_cancel(gpu, kernel, dtype):
         x = av.to(F32)
         assert torch.equal(mx.dequantize(mx.quantize(x, "e4m3"), F32), x)
         _check(mx.linear(x, w, out_dtype=dtype), u, (128 + k // 128) * U * size, None, None, dtype, kernel)
+
+
+# ------------------------------------------------------------------------------------------ sizes
+@pytest.mark.parametrize("m", [1, 17])
+def test_more_columns_than_a_launch_has_work_items_for(gpu, m):
+    """2^27 and some weight rows of 1000 columns: 64 GiB, eight waves a workgroup."""
+    n, k = (1 << 27) + 77, 1000
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info(gpu)[0] < 90 << 30:
+        pytest.skip("needs 90 GiB of device memory")
+    at = torch.tensor([0, 1, 15, 16, n // 2, (1 << 27) - 1, 1 << 27, n - 70, n - 17, n - 1])
+    a, av, some, wv = _operands(m, len(at), k, "e2m1", gpu)
+    data, scale = torch.zeros(n, 512, dtype=torch.uint8, device=gpu), torch.full((n, 32), 127, dtype=torch.uint8, device=gpu)
+    data[at.to(gpu)], scale[at.to(gpu)] = some.data, some.scale
+    y = mx.linear(a, mx.MXTensor(data, scale, "e2m1", k))
+    u, size = av @ wv.t().contiguous(), av.abs() @ wv.abs().t().contiguous()
+    _check(y[:, at.to(gpu)], u, (128 + 8) * U * size, None, None, BF16, "columns")
+    y[:, at.to(gpu)] = 0
+    assert not y.any()
+    del data, scale, y
+    torch.cuda.empty_cache()
