@@ -128,3 +128,29 @@ def test_more_columns_than_a_launch_has_work_items_for(gpu, m):
     assert not y.any()
     del data, scale, y
     torch.cuda.empty_cache()
+
+
+# ------------------------------------------------------------------------------------------ activations
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ["gelu", "quick_gelu"])
+@pytest.mark.parametrize("m,n", [(1, 4000), (300, 4000), (1, 30000), (4096, 4096), (4100, 4000)])
+def test_activations_of_exact_arguments(gpu, m, n, act, dtype):
+    """Products of zero rows: the argument is the bias."""
+    w, _ = _coded(n, 128, "e2m1", n, gpu, -3, 0)
+    x = mx.MXTensor(torch.zeros(m, 128, dtype=torch.uint8, device=gpu), torch.full((m, 4), 127, dtype=torch.uint8, device=gpu), "e4m3", 128)
+    g = torch.Generator().manual_seed(n)
+    bias = 26 * torch.rand(n, generator=g) - 13
+    bias[::7] *= 2.0 ** -6
+    bias[5:20] = torch.tensor([0.0, -0.0, 1e-30, -1e-30, 13.5, -40.0, 40.0, 1e4, -1e4, 1e30, -1e30, 3e38, -3e38, float("inf"), float("nan")])
+    u = bias.to(gpu).double()
+    y = mx.linear(x, w, bias=bias.to(gpu), act=act, out_dtype=dtype)
+    want = _activate(u, act)
+    assert torch.isnan(y[:, 19]).all() and torch.isinf(y[:, 18]).all()
+    far = want.abs() > torch.finfo(dtype).max
+    assert (y[:, far].double() == want[far].sign() * float("inf")).all()
+    fine = ~far & ~torch.isnan(want)
+    want, got = want[fine], y[:, fine].double()
+    tol = _act_error(want, dtype)
+    tol = tol + _half(dtype) * (want.abs() + tol) + float(torch.finfo(dtype).smallest_normal) * torch.finfo(dtype).eps
+    off = (got - want).abs() - tol
+    assert not (off > 0).any(), (off.max().item(), u[fine][int(off.max(0).values.argmax())].item())
