@@ -166,6 +166,16 @@ __global__ __launch_bounds__(256) void mx_dequant_kernel(const uint8_t* __restri
     if constexpr (FMT == MX_ROW_E4M3) s = ((const float*)scale)[row];
     else s = scale_value(((const uint8_t*)scale)[(size_t)row * (kp / 32) + c / 32]);
   };
+  // A block's scale is a power of two and the product exact; with a row's it has up to 28 bits, which reach 16 through an fp32 value rounded to
+  // odd: of the two neighbours the one whose last bit is set.
+  auto times = [](float a, float s) {
+    const float p = a * s;
+    if constexpr (FMT != MX_ROW_E4M3 || sizeof(T) == 4) return p;
+    const float rest = __builtin_fmaf(a, s, -p);
+    uint32_t b = __float_as_uint(p);
+    if ((rest > 0.0f || rest < 0.0f) && !(b & 1u)) b += (rest > 0.0f) == (p > 0.0f) ? 1u : 0xffffffffu;
+    return __uint_as_float(b);
+  };
   auto store = [&](long row, u32x2_t w, float s) {
     float v[8];
     if constexpr (FMT == MX_E2M1) {
@@ -179,10 +189,10 @@ __global__ __launch_bounds__(256) void mx_dequant_kernel(const uint8_t* __restri
     } else {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        v[4 * i] = __builtin_amdgcn_cvt_f32_fp8((int)w[i], 0) * s;
-        v[4 * i + 1] = __builtin_amdgcn_cvt_f32_fp8((int)w[i], 1) * s;
-        v[4 * i + 2] = __builtin_amdgcn_cvt_f32_fp8((int)w[i], 2) * s;
-        v[4 * i + 3] = __builtin_amdgcn_cvt_f32_fp8((int)w[i], 3) * s;
+        v[4 * i] = times(__builtin_amdgcn_cvt_f32_fp8((int)w[i], 0), s);
+        v[4 * i + 1] = times(__builtin_amdgcn_cvt_f32_fp8((int)w[i], 1), s);
+        v[4 * i + 2] = times(__builtin_amdgcn_cvt_f32_fp8((int)w[i], 2), s);
+        v[4 * i + 3] = times(__builtin_amdgcn_cvt_f32_fp8((int)w[i], 3), s);
       }
     }
     store_raw<T, WHOLE>(out + (size_t)row * k, c, k, raw_of<T>(v));

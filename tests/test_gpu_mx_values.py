@@ -154,3 +154,46 @@ def test_activations_of_exact_arguments(gpu, m, n, act, dtype):
     tol = tol + _half(dtype) * (want.abs() + tol) + float(torch.finfo(dtype).smallest_normal) * torch.finfo(dtype).eps
     off = (got - want).abs() - tol
     assert not (off > 0).any(), (off.max().item(), u[fine][int(off.max(0).values.argmax())].item())
+
+
+# ------------------------------------------------------------------------------------------ reading back
+def _rounded(v, dtype):
+    """float64 values, each the product of two numbers of at most 24 and 4 bits, to the nearest of the type, ties to even, in one rounding."""
+    bits, low = {BF16: (8, -133), F16: (11, -24), F32: (24, -149)}[dtype]
+    _, e = np.frexp(v)
+    unit = np.ldexp(1.0, np.maximum(e - bits, low))
+    v = np.rint(v / unit) * unit
+    return np.where(np.abs(v) > torch.finfo(dtype).max, np.sign(v) * np.inf, v)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols", [9, 128, 1001])
+def test_rows_with_one_scale_are_read_back_in_one_rounding(gpu, cols, dtype):
+    """Scales of any bits, and such that a product lies just beside a tie between two values of the type."""
+    r = np.random.RandomState(cols)
+    rows = 600
+    codes = r.randint(0, 256, (rows, ora.padded(cols))).astype(np.uint8)
+    codes[(codes & 127) == 127] = 0
+    codes[:, :8] = np.arange(0x38, 0x40)                                          # 1 .. 1.875
+    codes[:, cols:] = 0
+    scale = np.exp(r.uniform(-8, 4, rows)).astype(np.float32)
+    bits = {BF16: 8, F16: 11, F32: 23}[dtype]
+    tie = (2 * r.randint(2 ** (bits - 1), 2 ** bits, rows - 100) + 1) * 2.0 ** -bits
+    scale[100:] = (tie / (1 + r.randint(0, 8, rows - 100) / 8)).astype(np.float32)
+    q = mx.MXTensor(torch.from_numpy(codes).to(gpu), torch.from_numpy(scale).to(gpu), "e4m3_row", cols)
+    want = _rounded(ora.values(codes, scale, "e4m3_row", cols), dtype)
+    got = mx.dequantize(q, dtype).cpu().double().numpy()
+    assert np.array_equal(got, want), np.argwhere(got != want)[:5]
+
+
+def test_rows_with_scales_at_the_ends_of_their_range(gpu):
+    scale = np.array([0.0, -0.0, 1.0, np.float32(2.0 ** -149), np.float32(2.0 ** -130), np.float32(3e38), np.inf, np.nan], np.float32)
+    codes = np.tile(np.arange(128, dtype=np.uint8), (8, 1))
+    codes[:, 64:] |= 0x80
+    q = mx.MXTensor(torch.from_numpy(codes).to(gpu), torch.from_numpy(scale).to(gpu), "e4m3_row", 128)
+    with np.errstate(invalid="ignore"):
+        want = ora.values(codes, scale, "e4m3_row", 128)
+    for dtype in DTYPES:
+        got = mx.dequantize(q, dtype).cpu().double().numpy()
+        with np.errstate(invalid="ignore"):
+            assert np.array_equal(got, np.where(np.isfinite(want), _rounded(np.where(np.isfinite(want), want, 0.0), dtype), want), equal_nan=True)
