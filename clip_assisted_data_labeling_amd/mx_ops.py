@@ -21,7 +21,8 @@ NORMS = {"rms": 0, "layer": 1}
 ACTS = {None: -1, "quick_gelu": 0, "gelu": 1}
 _BLOCKS = {"e2m1": 0, "e4m3": 1}      # formats of a product's rows
 _WEIGHTS = {"e2m1": 0}                # and of its weights
-_MAX_ROWS = 1 << 30
+_MAX_ROWS = 1 << 30                   # what the library takes; checked here too, since an int argument keeps the low 32 bits of a larger number
+_MAX_COLS = 1 << 20
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
@@ -68,6 +69,8 @@ def _check_values(what: str, x: torch.Tensor, name: str = "x"):
     if len(shape) != 2 or shape[1] < 1:
         raise ValueError(f"{what}: expected {name} of shape [rows, cols], got {tuple(shape)}")
     rows, cols = shape
+    if cols > _MAX_COLS:
+        raise ValueError(f"{what}: at most {_MAX_COLS} columns, got {name} of shape {tuple(shape)}")
     ld, step = x.stride()
     if step != 1 and cols > 1:
         raise ValueError(f"{what}: the columns of {name} must lie side by side (stride 1), got strides {x.stride()}")
@@ -84,12 +87,14 @@ def _check_quantised(what: str, q: MXTensor, formats, name: str):
     code = formats.get(fmt)
     if code is None:
         raise ValueError(f"{what}: {name} must be one of {sorted(formats)}, got {fmt!r}")
+    if not 1 <= cols <= _MAX_COLS:
+        raise ValueError(f"{what}: {name} has {cols} columns (1 .. {_MAX_COLS})")
     kp = (cols + 127) // 128 * 128
     shape = data.shape
     rows = shape[0] if len(shape) == 2 else -1
     want, kind = ((rows, kp // 32), torch.uint8) if code != 2 else ((rows,), torch.float32)
     row_bytes = kp if code else kp // 2
-    if cols < 1 or rows < 0 or shape[1] != row_bytes or data.dtype is not torch.uint8 or scale.dtype is not kind or scale.shape != want:
+    if rows < 0 or shape[1] != row_bytes or data.dtype is not torch.uint8 or scale.dtype is not kind or scale.shape != want:
         raise ValueError(f"{what}: {name} of {cols} columns in {fmt} needs uint8 data of {row_bytes} bytes a row and {kind} scales {want}, "
                          f"got {data.dtype} {tuple(shape)} and {scale.dtype} {tuple(scale.shape)}")
     if not (data.is_contiguous() and scale.is_contiguous()):

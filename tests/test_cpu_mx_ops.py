@@ -125,3 +125,36 @@ def test_the_wrapper_refuses_more_rows_than_an_int_holds(monkeypatch, rows, out)
     q = mx.MXTensor(None, None, "e4m3", 64)
     with pytest.raises(ValueError, match="at most"):
         mx.linear(q, q)
+
+
+class _Wide:
+    """A tensor on a GPU of more columns than 32 bits hold, as far as the checks look at it."""
+    is_cuda, dtype, shape = True, torch.bfloat16, (1, (1 << 32) + 64)
+
+    def stride(self):
+        return (1 << 32) + 64, 1
+
+    def get_device(self):
+        return 0
+
+
+def test_the_wrapper_refuses_more_columns_than_an_int_holds():
+    x = _Wide()
+    for call in (lambda: mx.quantize(x), lambda: mx.norm_quantize(x, torch.ones(64)), lambda: mx.linear(x, _coded(64))):
+        with pytest.raises(ValueError, match="columns"):
+            call()
+    for cols in ((1 << 32) + 64, (1 << 20) + 1, 0, -64):
+        for call in (lambda: mx.dequantize(_coded(cols)), lambda: mx.linear(_coded(cols), _coded(64)), lambda: mx.linear(_coded(64), _coded(cols))):
+            with pytest.raises(ValueError, match="columns"):
+                call()
+
+
+def _coded(cols):
+    """Says that it has `cols` columns, on what would be a GPU."""
+    class Data:
+        is_cuda, dtype, shape, device = True, torch.uint8, (1, max(cols, 0) + 127 >> 7 << 6), "cuda:0"
+        is_contiguous, get_device = (lambda self: True), (lambda self: 0)
+
+    class Scale(Data):
+        shape = (1, max(cols, 0) + 127 >> 7 << 2)
+    return mx.MXTensor(Data(), Scale(), "e2m1", cols)
