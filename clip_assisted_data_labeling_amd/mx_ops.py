@@ -5,8 +5,9 @@ produces them and the product of such rows with 4-bit weights (include/clipenc.h
     h, q = norm_quantize(x, gamma, residual=r)                        # h = x + r;  q = rms norm of h, e4m3 in blocks
     y = linear(q, w, bias=b, act="gelu")                              # or linear(x, w): quantises x first
 
-The arithmetic runs in libclipenc_hip.so; there is no CPU path.  Calls are asynchronous on the current stream of the tensors'
-device, allocate only what they return (`linear` from values also a scratch) and may be captured into a graph.
+They have no backward pass: with gradients enabled, tensors that require one are refused.  The arithmetic runs in libclipenc_hip.so; there
+is no CPU path.  Calls are asynchronous on the current stream of the tensors' device, allocate only what they return (`linear` from
+values also a scratch) and may be captured into a graph.
 """
 from __future__ import annotations
 
@@ -46,6 +47,7 @@ class MXTensor(NamedTuple):
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
 _empty = torch.empty_strided
+_grad_enabled = torch.is_grad_enabled
 
 
 def _call(index: int, what: str, fn, *args) -> None:
@@ -57,6 +59,14 @@ def _call(index: int, what: str, fn, *args) -> None:
             rc = fn(*args, _raw_stream(index))
     if rc:
         _lib.check(rc, what)
+
+
+def _check_no_grad(what: str, *tensors) -> None:
+    """None of these operators has a backward pass: a gradient that the caller expects would be lost without a word."""
+    if _grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{what} has no backward pass: call it under torch.no_grad(), or with tensors that require no gradient")
 
 
 def _check_values(what: str, x: torch.Tensor, name: str = "x"):
@@ -132,6 +142,7 @@ def quantize(x: torch.Tensor, fmt: str = "e2m1") -> MXTensor:
     code = _BLOCKS.get(fmt)
     if code is None:
         raise ValueError(f"quantize: fmt must be 'e2m1' or 'e4m3', got {fmt!r}")
+    _check_no_grad("quantize", x)
     dt, index, rows, cols, ld = _check_values("quantize", x)
     q = _new(rows, cols, fmt, x.device)
     _call(index, "quantize", _lib.load().clipenc_op_quant_mx, x.data_ptr(), dt, rows, cols, ld, code, q[0].data_ptr(), q[1].data_ptr())
@@ -143,6 +154,7 @@ def dequantize(q: MXTensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor
     out_dt = _DTYPES.get(dtype)
     if out_dt is None:
         raise ValueError(f"dequantize: dtype must be bfloat16, float16 or float32, got {dtype}")
+    _check_no_grad("dequantize", q[1])                              # (a row's scale may be any float32 tensor)
     code, index, rows, cols = _check_quantised("dequantize", q, FORMATS, "q")
     data = q[0]
     out = _empty((rows, cols), (cols, 1), dtype=dtype, device=data.device)
@@ -158,6 +170,7 @@ def norm_quantize(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
     kind, code = NORMS.get(norm), FORMATS.get(fmt)
     if kind is None or code is None:
         raise ValueError(f"{what}: norm must be one of {sorted(NORMS)} and fmt one of {sorted(FORMATS)}, got {norm!r}, {fmt!r}")
+    _check_no_grad(what, x, weight, bias, residual)
     dt, index, rows, cols, ld = _check_values(what, x)
     device = x.device
     r = hp = None
@@ -189,8 +202,9 @@ def linear(x, w: MXTensor, bias: Optional[torch.Tensor] = None, act: Optional[st
         raise ValueError(f"{what}: act must be None, 'quick_gelu' or 'gelu', got {act!r}")
     if residual is not None and act is not None:
         raise ValueError(f"{what}: activation and residual are exclusive")
-    _, index, n, w_cols = _check_quantised(what, w, _WEIGHTS, "w")
     coded = isinstance(x, MXTensor)
+    _check_no_grad(what, None if coded else x, bias, residual)
+    _, index, n, w_cols = _check_quantised(what, w, _WEIGHTS, "w")
     if coded:
         fmt, x_index, rows, cols = _check_quantised(what, x, _BLOCKS, "x")
     else:

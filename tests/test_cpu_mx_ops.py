@@ -129,7 +129,7 @@ def test_the_wrapper_refuses_more_rows_than_an_int_holds(monkeypatch, rows, out)
 
 class _Wide:
     """A tensor on a GPU of more columns than 32 bits hold, as far as the checks look at it."""
-    is_cuda, dtype, shape = True, torch.bfloat16, (1, (1 << 32) + 64)
+    is_cuda, dtype, shape, requires_grad = True, torch.bfloat16, (1, (1 << 32) + 64), False
 
     def stride(self):
         return (1 << 32) + 64, 1
@@ -156,5 +156,23 @@ def _coded(cols):
         is_contiguous, get_device = (lambda self: True), (lambda self: 0)
 
     class Scale(Data):
+        requires_grad = False
         shape = (1, max(cols, 0) + 127 >> 7 << 2)
     return mx.MXTensor(Data(), Scale(), "e2m1", cols)
+
+
+def test_tensors_that_require_a_gradient_are_refused():
+    """Their gradient would be lost without a word; under no_grad they get as far as any CPU tensor."""
+    x, r, v, p = torch.zeros(2, 64), torch.zeros(2, 64), torch.ones(64), lambda t: torch.nn.Parameter(t.clone())
+    q = mx.MXTensor(torch.zeros(64, 64, dtype=torch.uint8), torch.zeros(64, 4, dtype=torch.uint8), "e2m1", 64)
+    row = mx.MXTensor(torch.zeros(2, 128, dtype=torch.uint8), p(v[:2]), "e4m3_row", 64)
+    calls = [lambda: mx.dequantize(row), lambda: mx.quantize(p(x)), lambda: mx.norm_quantize(p(x), v), lambda: mx.norm_quantize(x, p(v)), lambda: mx.norm_quantize(x, v, bias=p(v)),
+             lambda: mx.norm_quantize(x, v, residual=p(r)), lambda: mx.linear(p(x), q), lambda: mx.linear(x, q, bias=p(v)), lambda: mx.linear(q, q, bias=p(v)),
+             lambda: mx.linear(x, q, residual=p(r)), lambda: mx.linear(x * p(x), q)]
+    for call in calls:
+        with pytest.raises(ValueError, match="no backward"):
+            call()
+    with torch.no_grad():
+        for call in calls:
+            with pytest.raises(_lib.ClipencError, match="no CPU path"):
+                call()
