@@ -109,25 +109,69 @@ def test_sums_of_e4m3_rows_whose_large_products_cancel(gpu, kernel, dtype):
         _check(mx.linear(x, w, out_dtype=dtype), u, (128 + k // 128) * U * size, None, None, dtype, kernel)
 
 
-# ------------------------------------------------------------------------------------------ sizes
-@pytest.mark.parametrize("m", [1, 17])
-def test_more_columns_than_a_launch_has_work_items_for(gpu, m):
-    """2^27 and some weight rows of 1000 columns: 64 GiB, eight waves a workgroup."""
-    n, k = (1 << 27) + 77, 1000
-    torch.cuda.empty_cache()
-    if torch.cuda.mem_get_info(gpu)[0] < 90 << 30:
-        pytest.skip("needs 90 GiB of device memory")
-    at = torch.tensor([0, 1, 15, 16, n // 2, (1 << 27) - 1, 1 << 27, n - 70, n - 17, n - 1])
-    a, av, some, wv = _operands(m, len(at), k, "e2m1", gpu)
-    data, scale = torch.zeros(n, 512, dtype=torch.uint8, device=gpu), torch.full((n, 32), 127, dtype=torch.uint8, device=gpu)
-    data[at.to(gpu)], scale[at.to(gpu)] = some.data, some.scale
-    y = mx.linear(a, mx.MXTensor(data, scale, "e2m1", k))
+# ------------------------------------------------------------------------------------------ every kernel, every type of result
+@pytest.mark.parametrize("fmt", ["e2m1", "e4m3"])
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_every_kernel_every_type_and_epilogue(gpu, kernel, fmt):
+    m, n, k = KERNELS[kernel]
+    a, av, w, wv = _operands(m, n, k, fmt, gpu)
+    g = torch.Generator().manual_seed(k)
+    bias = (3 * torch.randn(n, generator=g)).to(gpu)
+    res = (50 * torch.randn(m, n, generator=g)).to(gpu)
     u, size = av @ wv.t().contiguous(), av.abs() @ wv.abs().t().contiguous()
-    _check(y[:, at.to(gpu)], u, (128 + 8) * U * size, None, None, BF16, "columns")
-    y[:, at.to(gpu)] = 0
-    assert not y.any()
-    del data, scale, y
-    torch.cuda.empty_cache()
+    with_bias, count = u + bias.double(), 128 + ora.padded(k) // 128 + 2
+    pre = count * U * (size + bias.double().abs())
+    for dtype in DTYPES:
+        _check(mx.linear(a, w, out_dtype=dtype), u, count * U * size, None, None, dtype, dtype)
+        for act in (None, "gelu", "quick_gelu"):
+            _check(mx.linear(a, w, bias=bias, act=act, out_dtype=dtype), with_bias, pre, act, None, dtype, (dtype, act))
+        r = res.to(dtype)
+        _check(mx.linear(a, w, bias=bias, residual=r, out_dtype=dtype), with_bias, pre, None, r, dtype, (dtype, "residual"))
+
+
+@pytest.mark.parametrize("fmt", ["e2m1", "e4m3"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k", [(301, 1101, 200), (2885, 1003, 601), (4100, 4090, 300)])
+def test_values_through_tiles_are_quantize_and_linear(gpu, m, n, k, dtype, fmt):
+    _, _, w, wv = _operands(1, n, k, fmt, gpu)
+    x = (0.5 * torch.randn(m, k, generator=torch.Generator().manual_seed(m))).to(dtype).to(gpu)
+    q = mx.quantize(x, fmt)
+    av = torch.from_numpy(ora.values(ora.unpack(q.data.cpu().numpy(), fmt), q.scale.cpu().numpy(), fmt, k)).to(gpu)
+    u, size = av @ wv.t().contiguous(), av.abs() @ wv.abs().t().contiguous()
+    y = mx.linear(x, w, x_fmt=fmt)
+    _check(y, u, (128 + ora.padded(k) // 128) * U * size, None, None, dtype, "values")
+    assert torch.equal(y, mx.linear(q, w, out_dtype=dtype))
+
+
+@pytest.mark.parametrize("fmt", ["e2m1", "e4m3"])
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_residual_in_place_and_nothing_behind_the_last_row(gpu, kernel, fmt):
+    lib, s = _lib.load(), _lib.current_stream_ptr(gpu)
+    m, n, k = KERNELS[kernel]
+    a, _, w, _ = _operands(m, n, k, fmt, gpu)
+    for code, dtype in enumerate(DTYPES):
+        res = (50 * torch.randn(m, n, generator=torch.Generator().manual_seed(n))).to(dtype).to(gpu)
+        want = mx.linear(a, w, residual=res, out_dtype=dtype)
+        out = torch.full((m + 2, n), 7.0, device=gpu, dtype=dtype)
+        out[:m] = res
+        _lib.check(lib.clipenc_op_gemm_mx(a.data.data_ptr(), a.scale.data_ptr(), mx.FORMATS[fmt], w.data.data_ptr(), w.scale.data_ptr(), m, n, k, None, -1, out.data_ptr(),
+                                          out.data_ptr(), code, s), "gemm")
+        assert torch.equal(out[:m], want) and (out[m:] == 7.0).all()
+
+
+@pytest.mark.parametrize("fmt", ["e2m1", "e4m3"])
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_a_block_that_is_not_finite_is_in_its_own_row_or_column_only(gpu, kernel, fmt):
+    m, n, k = KERNELS[kernel]
+    a, _, w, _ = _operands(m, n, k, fmt, gpu)
+    a.scale[m // 2, 1] = 255
+    w.scale[n // 3, 0] = 255
+    want = torch.zeros(m, n, dtype=torch.bool, device=gpu)
+    want[m // 2] = True
+    want[:, n // 3] = True
+    for dtype in (BF16, F32):
+        for act in (None, "gelu", "quick_gelu"):
+            assert torch.equal(torch.isnan(mx.linear(a, w, act=act, out_dtype=dtype)), want)
 
 
 # ------------------------------------------------------------------------------------------ activations
@@ -163,7 +207,7 @@ def _rounded(v, dtype):
     _, e = np.frexp(v)
     unit = np.ldexp(1.0, np.maximum(e - bits, low))
     v = np.rint(v / unit) * unit
-    return np.where(np.abs(v) > torch.finfo(dtype).max, np.sign(v) * np.inf, v)
+    return np.where(np.abs(v) > torch.finfo(dtype).max, np.copysign(np.inf, v), v)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -197,3 +241,24 @@ def test_rows_with_scales_at_the_ends_of_their_range(gpu):
         got = mx.dequantize(q, dtype).cpu().double().numpy()
         with np.errstate(invalid="ignore"):
             assert np.array_equal(got, np.where(np.isfinite(want), _rounded(np.where(np.isfinite(want), want, 0.0), dtype), want), equal_nan=True)
+
+
+# ------------------------------------------------------------------------------------------ sizes
+@pytest.mark.parametrize("m", [1, 17])
+def test_more_columns_than_a_launch_has_work_items_for(gpu, m):
+    """2^27 and some weight rows of 1000 columns: 64 GiB, eight waves a workgroup."""
+    n, k = (1 << 27) + 77, 1000
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info(gpu)[0] < 90 << 30:
+        pytest.skip("needs 90 GiB of device memory")
+    at = torch.tensor([0, 1, 15, 16, n // 2, (1 << 27) - 1, 1 << 27, n - 70, n - 17, n - 1])
+    a, av, some, wv = _operands(m, len(at), k, "e2m1", gpu)
+    data, scale = torch.zeros(n, 512, dtype=torch.uint8, device=gpu), torch.full((n, 32), 127, dtype=torch.uint8, device=gpu)
+    data[at.to(gpu)], scale[at.to(gpu)] = some.data, some.scale
+    y = mx.linear(a, mx.MXTensor(data, scale, "e2m1", k))
+    u, size = av @ wv.t().contiguous(), av.abs() @ wv.abs().t().contiguous()
+    _check(y[:, at.to(gpu)], u, (128 + 8) * U * size, None, None, BF16, "columns")
+    y[:, at.to(gpu)] = 0
+    assert not y.any()
+    del data, scale, y
+    torch.cuda.empty_cache()
