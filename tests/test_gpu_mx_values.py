@@ -200,6 +200,30 @@ def test_activations_of_exact_arguments(gpu, m, n, act, dtype):
     assert not (off > 0).any(), (off.max().item(), u[fine][int(off.max(0).values.argmax())].item())
 
 
+# ------------------------------------------------------------------------------------------ norm
+@pytest.mark.parametrize("fmt", ["e2m1", "e4m3", "e4m3_row"])
+@pytest.mark.parametrize("rows,cols", [(1, 64), (3, 1000), (5, 1280), (3000, 1280), (4, 2400), (2, 9000)])
+def test_norm_of_values_beside_a_tie_has_the_codes_of_64_bits(gpu, rows, cols, fmt):
+    """Rows of +-1, whose root mean square is 1: y = +-gamma + beta with gamma a tie of the format and beta +-2^-30 of it, which fp32 does not hold."""
+    r = np.random.RandomState(cols)
+    kind = "e2m1" if fmt == "e2m1" else "e4m3"
+    grid = ora.grid(kind)
+    ties = (grid[1:] + grid[:-1]) / 2
+    gamma = ties[r.randint(1, len(ties), cols)]
+    gamma[::32] = grid[-1]                                                        # every block's and the row's largest: scales of 1
+    beta = gamma * 2.0 ** -30 * r.choice([-1.0, 1.0], cols)
+    beta[::32] = 0.0
+    sign = r.choice([-1.0, 1.0], (rows, cols))
+    y = sign * gamma + beta
+    dev = lambda v, t: torch.from_numpy(v).to(t).to(gpu)                          # noqa: E731
+    _, q = mx.norm_quantize(dev(sign, BF16), dev(gamma, F32), bias=dev(beta, F32), eps=0.0, fmt=fmt)
+    codes = ora.unpack(q.data.cpu().numpy(), fmt)[:, :cols]
+    assert (q.scale == 1.0).all() if fmt == "e4m3_row" else (q.scale[:, :cols // 32] == 127).all()
+    want = ora.nearest_code(np.abs(y), kind) | np.where(np.signbit(y), 8 if fmt == "e2m1" else 128, 0)
+    assert np.array_equal(codes, want)
+    assert (want != (ora.nearest_code(np.float32(np.abs(y)).astype(np.float64), kind) | np.where(np.signbit(y), 8 if fmt == "e2m1" else 128, 0))).any()
+
+
 # ------------------------------------------------------------------------------------------ reading back
 def _rounded(v, dtype):
     """float64 values, each the product of two numbers of at most 24 and 4 bits, to the nearest of the type, ties to even, in one rounding."""
