@@ -573,10 +573,10 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void mx_gemm_kernel(const MxGemmPa
 // Few rows, or few columns: 16 columns n a workgroup, whose waves share K and add their sums up in LDS, in wave order.  Fragments come straight from
 // memory -- each byte of W is read once, and there is nothing to wait for but that one read: a tile walk of the same product pays a
 // memory latency a stage.  SRC: quantised rows (MX_E2M1 / MX_E4M3), or values of type T that the lanes quantise themselves, with the
-// codes of clipenc_op_quant_mx; each workgroup does it again, so beyond MX_VALUE_COLS columns it has 64 of them (12 800 x 5120, one row:
-// 15 us instead of 24; 4096 x 1024, whose workgroups are then a quarter of the CUs: 6.3 instead of 4.5).
-// One row of 8192 x 1664 takes 4.2 us from codes, whose 7 MB of weights are 1.4 us of HBM and whose launch and one trip to memory are the
-// rest; 12 800 x 5120 (33 MB) 11.7 us, 2.9 TB/s.
+// codes of clipenc_op_quant_mx; each workgroup does it again, so beyond MX_VALUE_COLS columns it has 64 of them (12 800 x 5120, one row in
+// e4m3: 15 us instead of 26; 4096 x 1024, whose workgroups are then a quarter of the CUs: 5.9 instead of 3.9).
+// One row of 8192 x 1664 takes 3.7 us from codes, whose 7 MB of weights are 1.4 us of HBM and whose launch and one trip to memory are the
+// rest; 12 800 x 5120 (35 MB) 11 us, 3.2 TB/s.
 struct MxFewParams {
   MxGemmParams g;
   const void* x; long ld_x; int k;                // values: [M] rows of k
@@ -787,24 +787,26 @@ hipError_t launch(const MxGemmParams& p, hipStream_t stream) {
   return hipGetLastError();
 }
 
-// Fewer than a 256 x 256 tile a CU.  64 x 64 tiles while the CUs hold them in one go or nearly (two a CU, a third one joins late); beyond that
-// 128 x 128: 5120 columns of 577 / 1154 rows, e4m3: 19 / 25 us in 64 x 64, 15 / 17 in 128 x 128 -- in eight waves with four stages in LDS while
-// they are at most one a CU, and latency is what a stage costs, else in four waves, two workgroups a CU.  (e4m3: waves of 32 x 64, which
-// part each row fragment for four products instead of two: 46 -> 40 us at 2885 x 4001 -> 1003.)
+constexpr int CUS = 256;                // (a device with fewer CUs only takes its turns earlier)
+// Fewer than a 256 x 256 tile a CU.  64 x 64 tiles while the CUs hold them in one go, two a CU; a third one on some of them costs as much as
+// one on each, and 128 x 128 tiles then take less time (e2m1 / e4m3, us in 64 x 64 and in 128 x 128:  448 tiles, 400 rows x 1024 -> 4096, 6.9 / 11.6
+// and 7.7 / 13.3;  494, 1154 x 8192 -> 1664, 26 / 58 and 33 / 71;  528, 2056 x 1024 -> 1024, 8.7 / 15.7 and 7.7 / 13.1;  560, 400 x 1280 -> 5120,
+// 9.9 / 18.5 and 8.5 / 15.5;  640, 577 x 1024 -> 4096, 9.1 / 16.0 and 10.4 / 15.6, the one that loses;  832, 770 x 1024 -> 4096, 10.7 / 19.4 and
+// 8.1 / 13.8).  128 x 128: eight waves with four stages in LDS while they are at most one a CU, and latency is what a stage costs, else four waves, two
+// workgroups a CU.  (e4m3: waves of 32 x 64, which part each row fragment for four products instead of two: 46 -> 40 us at 2885 x 4001 -> 1003.)
 template <int AF>
 hipError_t small_tiles(const MxGemmParams& p, hipStream_t stream) {
   const long tiles64 = (long)((p.M + 63) / 64) * ((p.N + 63) / 64), tiles128 = (long)((p.M + 127) / 128) * ((p.N + 127) / 128);
-  if (tiles64 <= 704) return launch<AF, 64, 64, 2, 2, 4, true>(p, stream);
+  if (tiles64 <= 2 * CUS) return launch<AF, 64, 64, 2, 2, 4, true>(p, stream);
   if (tiles128 > 256) return launch<AF, 128, 128, 2, 2, 2, false>(p, stream);
   if constexpr (AF == A_E4M3) return launch<AF, 128, 128, 4, 2, 4, true>(p, stream);
   else return launch<AF, 128, 128, 2, 4, 4, true>(p, stream);
 }
 
 // The few-row kernel: up to 16 rows; up to 48 while its workgroups are at most two a CU (e2m1 / e4m3, 48 rows: 8192 columns of 1664
-// 5.9 / 10.1 us, in 64 x 64 tiles 8.5 / 11.9; 12 800 columns of 5120 28 / 47 against 16 / 27); more rows while its workgroups of 64 rows x
-// 16 columns are at most one a CU -- a long K is then shared by eight waves instead of walked by four (256 x 4096 -> 1024 9.8 / 13.3 us
-// against 11.1 / 19.1; 384 rows 16.5 / 24.6 against 11.2 / 19.2).
-constexpr int CUS = 256;                // (a device with fewer CUs only takes its turns earlier)
+// 5.4 / 10.8 us, in 64 x 64 tiles 7.8 / 13.0; 12 800 columns of 5120 28 / 47 against 15 / 32); more rows while its workgroups of 64 rows x
+// 16 columns are at most one a CU -- a long K is then shared by eight waves instead of walked by four (256 x 4096 -> 1024 9.5 / 14.1 us
+// against 10.5 / 24.3; 384 rows 16.0 / 25.9 against 10.6 / 24.2).
 inline bool few(const MxGemmParams& p) { return p.M <= 16 || (long)((p.M + 63) / 64) * ((p.N + 15) / 16) <= (p.M <= 48 ? 2 * CUS : CUS); }
 template <int AF>
 hipError_t few_rows(const MxGemmParams& p, hipStream_t stream) {

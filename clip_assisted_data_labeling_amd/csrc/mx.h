@@ -11,13 +11,13 @@
 enum { MX_E2M1 = 0, MX_E4M3 = 1, MX_ROW_E4M3 = 2 };
 enum { MX_DT_BF16 = 0, MX_DT_F16 = 1, MX_DT_F32 = 2 };
 enum { MX_NORM_RMS = 0, MX_NORM_LAYER = 1 };
-#define MX_NORM_MAX_K 16384             // widest row of the norm: 1024 threads hold it in registers, 16 values each
+#define MX_NORM_MAX_K 16384             // widest row of the norm: 512 threads hold it in registers, 32 values each
 
 static inline int mx_kp(int k) { return (k + 127) / 128 * 128; }
 // Whether a product quantises its rows itself, one launch instead of two, in every workgroup again: up to 16 rows, and up to 64 while the
-// workgroups of 16 x 16 results are two a CU or fewer (4096 x 1024, e4m3, GPU time of 1 / 32 rows: 4.5 / 6.4 us, in two launches 5.6 / 7.3;
-// 5120 x 1280, 24 rows: 9.9 against 8.1) -- and no more than 2^26 weights, whose sweep would be held up by it (12 800 x 5120, 1 / 16 rows:
-// 15 / 16 us against 14 / 21; 8192 x 8192: 20 / 24 against 12 / 18).
+// workgroups of 16 x 16 results are two a CU or fewer (4096 x 1024, e4m3, GPU time of 1 / 32 rows: 3.9 / 6.0 us, in two launches 5.0 / 6.6;
+// 5120 x 1280, 24 rows: 9.8 against 7.5) -- and fewer than 2^26 weights, whose sweep would be held up by it (12 800 x 5120, 1 / 16 rows:
+// 15 / 16 us against 14 / 21; 8192 x 8192: 21 / 26 against 12 / 18).
 static inline bool mx_takes_values(int m, int n, int k) {
   return (m <= 16 || (m <= 64 && (long)((m + 15) / 16) * ((n + 15) / 16) <= 512)) && (long)n * k < 1l << 26;
 }
