@@ -109,6 +109,40 @@ def test_sums_of_e4m3_rows_whose_large_products_cancel(gpu, kernel, dtype):
         _check(mx.linear(x, w, out_dtype=dtype), u, (128 + k // 128) * U * size, None, None, dtype, kernel)
 
 
+@pytest.mark.parametrize("fmt", ["e2m1", "e4m3"])
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_sums_whose_large_products_cancel_far_apart(gpu, kernel, fmt):
+    """Blocks 2^12 times the others cancel against another block of the same or of another K step."""
+    m, n, k = KERNELS[kernel]
+    k = max(256, ora.padded(k))
+    r = np.random.RandomState(n)
+    top, sign = (8, 8) if fmt == "e2m1" else (128, 128)
+    codes = r.randint(0, top // 2, (m, k)).astype(np.uint8)
+    scale, wscale = np.full((m, k // 32), 127, np.uint8), np.full((n, k // 32), 127, np.uint8)
+    wcodes = r.randint(0, 16, (n, k)).astype(np.uint8)
+    for at, to in ((0, 2), (1, 5)):                                               # of one step, of two
+        codes[:, to * 32:to * 32 + 32] = codes[:, at * 32:at * 32 + 32] | sign
+        wcodes[:, to * 32:to * 32 + 32] = wcodes[:, at * 32:at * 32 + 32]
+        scale[:, [at, to]] += 12
+    a, w = _lay_out(codes, scale, fmt, k, gpu), _lay_out(wcodes, wscale, "e2m1", k, gpu)
+    av, wv = (torch.from_numpy(ora.values(c, s, f, k)).to(gpu) for c, s, f in ((codes, scale, fmt), (wcodes, wscale, "e2m1")))
+    u, size = av @ wv.t().contiguous(), av.abs() @ wv.abs().t().contiguous()
+    for dtype in DTYPES:
+        _check(mx.linear(a, w, out_dtype=dtype), u, (128 + k // 128) * U * size, None, None, dtype, kernel)
+
+
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_nan_codes_of_e4m3_rows_are_in_their_own_row_only(gpu, kernel):
+    m, n, k = KERNELS[kernel]
+    a, _, w, _ = _operands(m, n, k, "e4m3", gpu)
+    a.data[m // 2, k - 1] = 0x7F
+    a.data[m - 1, 3] = 0xFF
+    want = torch.zeros(m, n, dtype=torch.bool, device=gpu)
+    want[m // 2] = want[m - 1] = True
+    for dtype in DTYPES:
+        assert torch.equal(torch.isnan(mx.linear(a, w, out_dtype=dtype)), want)
+
+
 # ------------------------------------------------------------------------------------------ every kernel, every type of result
 @pytest.mark.parametrize("fmt", ["e2m1", "e4m3"])
 @pytest.mark.parametrize("kernel", KERNELS)
