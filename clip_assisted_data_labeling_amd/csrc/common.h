@@ -42,7 +42,7 @@ static inline float host_bf16_to_f32(uint16_t h) {
 // erfc(z), z >= 0, by Abramowitz & Stegun 7.1.26:  t = 1 / (1 + p z),  erfc(z) = t (a1 + t (a2 + t (a3 + t (a4 + t a5)))) exp(-z^2),
 // |error| <= 1.5e-7 -- three decimal digits under the bf16 / e4m3 rounding of the result.  With q = erfc(|u| / sqrt 2):
 // GELU(u) = u - u q / 2 for u >= 0 and u q / 2 for u < 0, i.e. max(u, 0) - |u q / 2|.  16 issue slots (two of them transcendental)
-// where libdevice's erff is a branchy ~45: the erf-GELU FC1 epilogue was 22 % slower than the QuickGELU one.
+// where the device library's erff is a branchy ~45: the erf-GELU FC1 epilogue was 22 % slower than the QuickGELU one.
 __device__ __forceinline__ float ce_gelu_erf(float u) {
   const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(__builtin_fabsf(u), 0.3275911f * 0.70710678118654752f, 1.0f));
   float pl = __builtin_fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);

@@ -25,9 +25,10 @@
 // steps -- so that a lane holds the scales of 16 rows and a period in ONE word.
 //
 // Measured, 256 x 256 tiles:  16 384 x 8192 -> 4096  e2m1 271 us (4.05 PFLOP/s), e4m3 784 us (1.4, of MFMAs in two bands 2.8);  65 536 x 4096
-// -> 1024 in e2m1 160 us (3.4), 65 792 in e4m3 434 us (1.27); the bare instruction reaches 7.7 and 4.5.  Long e4m3 rows are bound by the
-// matrix pipe (one MFMA a fragment pair, whose sums the cut above would hold in 14 bits: 402 and 242 us).  A short K is bound by the way
-// out: 65 792 x 1024 -> 4096 in e2m1 with QuickGELU 253 us, 539 MB of results.
+// -> 1024 in e2m1 160 us (3.4), 65 792 in e4m3 434 us (1.27); the bare instruction reaches 7.7 and 4.5.  Over long e4m3 rows the matrix pipe is
+// busy 0.53 of the time, and waits at the barriers and for a stage's first fragments; one MFMA a fragment pair, whose sums the cut above
+// would hold in 14 bits, took 402 and 242 us.  A short K is bound by the way out: 65 792 x 1024 -> 4096 in e2m1 with QuickGELU 255 us, 539 MB
+// of results.
 #include <type_traits>
 
 #include "common.h"

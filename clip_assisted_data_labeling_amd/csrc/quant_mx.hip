@@ -16,9 +16,9 @@
 
 namespace {
 
-// 65 792 x 4096 of bf16 to e2m1 and back, 682 MB each: 117 us (5.8 TB/s) and 137 us (5.0).  Quantising wants many short workgroups -- one row
-// a thread and step: 256 workgroups a CU 117 us, 64 131; four rows in flight and 16 a CU 154 --, reading back few long ones: four rows in
-// flight and 8 a CU 137 us, 16 a CU 145, one row 182.
+// 65 792 x 4096 of bf16 to e2m1 and back, 682 MB each, one pass behind the other: 116 us (5.9 TB/s) and 136 us (5.0).  Quantising wants many short
+// workgroups -- one row a thread and step: 256 workgroups a CU 116 us, 64 131; four rows in flight and 16 a CU 154 --, reading back few long
+// ones: four rows in flight and 8 a CU 136 us, 16 a CU 141, one row 174 (e4m3: 159, 164, 151).
 constexpr int QUANT_BLOCKS = 256 * 256, DEQUANT_ROWS = 4, DEQUANT_BLOCKS = 256 * 8;
 
 typedef __attribute__((ext_vector_type(4))) uint32_t u32x4_t;

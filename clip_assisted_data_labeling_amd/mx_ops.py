@@ -193,9 +193,9 @@ def norm_quantize(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
 
 def linear(x, w: MXTensor, bias: Optional[torch.Tensor] = None, act: Optional[str] = None, residual: Optional[torch.Tensor] = None,
            out_dtype: Optional[torch.dtype] = None, x_fmt: str = "e4m3") -> torch.Tensor:
-    """act(x . w^T + bias) + residual, [rows, out].  x: an MXTensor ("e4m3" or "e2m1") or values [rows, cols], which are quantised to
-    x_fmt first; w: e2m1 [out, cols]; bias float32 [out]; act None, "quick_gelu" or "gelu" (erf), not together with a residual;
-    residual [rows, out] of out_dtype (default: the values' type, bf16 for an MXTensor)."""
+    """act(x . w^T + bias) + residual, [rows, out], summed in fp32 and rounded once.  x: an MXTensor ("e4m3" or "e2m1") or values
+    [rows, cols], which are quantised to x_fmt first; w: e2m1 [out, cols]; bias float32 [out]; act None, "quick_gelu" or "gelu" (erf),
+    not together with a residual; residual [rows, out] of out_dtype (default: the values' type, bf16 for an MXTensor)."""
     what = "linear"
     act_code = ACTS.get(act)
     if act_code is None:

@@ -376,12 +376,12 @@ int clipenc_op_dequant_mx(const void* q_dev, const void* scale_dev, int fmt, lon
  *       (h - mean(h)) * gamma / sqrt(var(h) + eps) + beta           CLIPENC_NORM_LAYER       (beta_dev may be NULL)
  * and y in fmt (any of the three).  gamma / beta: float [k]; k <= 16384; ld_in / ld_resid in elements; h_out_dev may be in_dev or
  * resid_dev where that one's rows are k elements apart.  Sums, the row's factor and y are formed
- * in 64 bits and y is rounded once, to its few (beyond fp32's range: not finite). */
+ * in 64 bits and y is rounded once, to its few (below 2^-126: by way of fp32's subnormal numbers; beyond fp32's range: not finite). */
 int clipenc_op_norm_quant_mx(const void* in_dev, int in_dtype, long n_rows, int k, long ld_in, const void* resid_dev, long ld_resid, int norm,
                              const float* gamma_dev, const float* beta_dev, float eps, int fmt, void* h_out_dev, void* out_dev,
                              void* scale_dev, void* stream);
 /* out[m][n] = act(A . W^T + bias[n]) + resid[m][n]:  A [m] rows of a_fmt (CLIPENC_MX_E2M1 / _E4M3), W [n] rows of CLIPENC_MX_E2M1, both of k
- * columns; products and sums in fp32, one rounding to out_dtype.  bias_dev (float [n]) and resid_dev ([m][n] of out_dtype, may be
+ * columns; products and sums in fp32 for every type, one rounding to out_dtype.  bias_dev (float [n]) and resid_dev ([m][n] of out_dtype, may be
  * out_dev) may be NULL; act: -1 none, CLIPENC_ACT_*; not both act and resid. */
 int clipenc_op_gemm_mx(const void* a_dev, const void* a_scale_dev, int a_fmt, const void* w_dev, const void* w_scale_dev, int m, int n, int k,
                        const float* bias_dev, int act, const void* resid_dev, void* out_dev, int out_dtype, void* stream);
