@@ -5,6 +5,7 @@ Tolerances, u = 2^-24, half(t) = torch.finfo(t).eps / 2.
   sums          products of e2m1 / e4m3 values and powers of two are exact in fp32; a K step of 128 adds at most 128 roundings and each further step
                 one, none larger than u times the products' magnitudes, in whatever order and for whatever type of result; then two fp32 roundings
                 (bias, residual) and one to the result's type
+                (test_gpu_mx_ops.py allows e4m3 rows with 16-bit results, and the norm's codes, more than they now need)
   activations   of an exact argument, relative.  16-bit results: their own half step and 2^-14 (a fit good to 2^-15.1, and exp2's argument,
                 at most 128 with two roundings of u: 256 u ln 2 < 2^-16).  fp32: 16 u (exp2 and rcp 2 u each, the fit and its
                 eight steps 6 u, four products and sums 4 u; the exponential's argument is carried in two floats).  Results below 2^-120 may be
